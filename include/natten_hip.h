@@ -359,6 +359,105 @@ int natten_hip_rpb_av_backward(const natten_problem_t *p,
                                void *dv, const natten_layout_t *ldv,
                                void *stream);
 
+/* Rotary positions (no counterpart in the reference).  A pair (u, v) of a
+ * head at coordinate x turns by t = 2 pi x f:
+ *   (u', v') = magnitude * (u cos t - v sin t, u sin t + v cos t),
+ * t negated with `inverse` (the gradient).  Axis a of `axes` owns dims
+ * [a n, (a + 1) n), n = turned / axes; pair j of an axis is dims (j, j + n/2)
+ * of its share, or (2j, 2j + 1) when interleaved.  Dims from `turned` on are
+ * copied.  turns[j], j < n / 2: f as an unsigned 64-bit fraction of a turn
+ * (device memory).  positions (device, position_bits 32 or 64) holds a
+ * coordinate per token and axis at element strides {batch, token, axis},
+ * tokens row-major over the grid; with position_bits 0 (positions NULL) a
+ * token's coordinates are its indices on the last `axes` axes of the grid.
+ * heads_q or heads_k may be 0 (operands NULL): one tensor alone.  Outputs
+ * must not overlap inputs. */
+typedef struct {
+    int32_t batch;
+    int32_t length[3];     /* token grid, padded in front with 1 */
+    int32_t heads_q;
+    int32_t heads_k;
+    int32_t dim;           /* head dim of q and k, at most 256 */
+    int32_t dtype;         /* natten_dtype_t */
+    int32_t axes;          /* 1..3 */
+    int32_t turned;        /* dims turned: a multiple of 2 * axes, 0..dim */
+    int32_t interleaved;
+    int32_t inverse;
+    float magnitude;
+    int32_t position_bits; /* 0, 32 or 64 */
+    int64_t position_stride[3];
+} natten_rotary_t;
+
+int natten_hip_rotary(const natten_rotary_t *r, const uint64_t *turns,
+                      const void *positions,
+                      const void *q, const natten_layout_t *lq,
+                      void *q_out, const natten_layout_t *lqo,
+                      const void *k, const natten_layout_t *lk,
+                      void *k_out, const natten_layout_t *lko,
+                      void *stream);
+
+/* A paged cache (no counterpart in the reference): token j of sequence b is
+ * slot j % page_size of page table[b * table_stride + j / page_size].  Keys
+ * are [pages, page_size, heads_kv, dim_qk] and values [.., dim_v] at element
+ * strides {page, slot, head}, head dims contiguous.  A table entry outside
+ * [0, pages), like a position past the table's width, names no page: its
+ * tokens are not written, and no query attends to them.
+ * seq_lens[b] counts the tokens of the sequence with the new ones; the last
+ * new_lens[b] (clamped to [0, tokens]; NULL: `tokens`) of them are new, token
+ * i of the call at position seq_lens[b] - new_lens[b] + i.  table, seq_lens
+ * and new_lens are int32 device memory and read on the stream; the call never
+ * waits for the device. */
+typedef struct {
+    int32_t batch;
+    int32_t tokens;        /* new tokens per sequence, padded */
+    int32_t heads_q;
+    int32_t heads_kv;      /* heads_q % heads_kv == 0 */
+    int32_t dim_qk;        /* at most 256 */
+    int32_t dim_v;         /* at most 256 */
+    int32_t dtype;         /* natten_dtype_t */
+    int32_t pages;
+    int32_t page_size;
+    int32_t table_width;   /* entries per sequence */
+    int64_t table_stride;
+    int64_t key_stride[3];   /* page, slot, head */
+    int64_t value_stride[3];
+    int32_t kernel;        /* attention: window in keys; 0: all earlier keys */
+    int32_t dilation;
+    float scale;
+} natten_paged_t;
+
+/* New tokens into the cache: keys turned by their positions (r: turned,
+ * interleaved and magnitude are read, turns as above; r NULL: as they are),
+ * values copied.  q (may be NULL) is turned alike into q_out, zeros at
+ * padding tokens.  A page that takes new tokens must belong to one sequence. */
+int natten_hip_paged_append(const natten_paged_t *p, const natten_rotary_t *r,
+                            const uint64_t *turns,
+                            const int32_t *table, const int32_t *seq_lens,
+                            const int32_t *new_lens,
+                            const void *k, const natten_layout_t *lk,
+                            const void *v, const natten_layout_t *lv,
+                            const void *q, const natten_layout_t *lq,
+                            void *q_out, const natten_layout_t *lqo,
+                            void *key_pages, void *value_pages,
+                            void *stream);
+
+/* Attention of the new tokens over the cache: the query at position p attends
+ * to keys p - t * dilation >= 0, t < kernel (kernel 0: all of 0..p).  out
+ * [B, tokens, Hq, dim_v] and lse (fp32, natural log) get zeros and -inf at
+ * padding tokens and at rows without keys.  `work` holds
+ * natten_hip_paged_workspace bytes, 16-byte aligned (not needed when 0); it
+ * is this call's until its kernels end. */
+int64_t natten_hip_paged_workspace(const natten_paged_t *p);
+int natten_hip_paged_forward(const natten_paged_t *p,
+                             const int32_t *table, const int32_t *seq_lens,
+                             const int32_t *new_lens,
+                             const void *q, const natten_layout_t *lq,
+                             const void *key_pages, const void *value_pages,
+                             void *out, const natten_layout_t *lo,
+                             float *lse, const natten_layout_t *llse,
+                             void *work, int64_t work_bytes,
+                             void *stream);
+
 /* Per-kernel timing (no counterpart in the reference; for benchmarks and
  * profiling).  While enabled, every kernel launch of the library is bracketed
  * by two HIP events on its stream.  natten_hip_profile_read waits for the

@@ -864,3 +864,238 @@ int natten_hip_neighborhood_map(const natten_problem_t* p, int64_t* flat, uint8_
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// rotary positions and the paged cache
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// Elements of a 16-byte (8-byte for some 16-bit heads) vector that divides an
+// axis's pairs and the copied dims, with every operand aligned for it; else 1.
+int rotary_vec(int dtype, int dim, int turned, int axes, int dim_v, std::initializer_list<Run> ts) {
+    for (int vec : {16 / elem_size(dtype), 4}) {
+        if (turned % (2 * axes * vec) || (dim - turned) % vec || dim_v % vec) continue;
+        bool ok = true;
+        for (auto& t : ts) {
+            if (!t.ptr) continue;
+            if (reinterpret_cast<uintptr_t>(t.ptr) % (vec * elem_size(dtype))) ok = false;
+            const natten_layout_t* l = t.lay;
+            if (l->batch % vec || l->axis[0] % vec || l->axis[1] % vec || l->axis[2] % vec || l->head % vec) ok = false;
+        }
+        if (ok) return vec;
+    }
+    return 1;
+}
+
+int check_turn(const natten_rotary_t* r, int dim, const uint64_t* turns) {
+    if (r->axes < 1 || r->axes > 3) return fail(NATTEN_ERR_INVALID, "axes must be 1..3, got %d", r->axes);
+    if (r->turned < 0 || r->turned > dim || r->turned % (2 * r->axes))
+        return fail(NATTEN_ERR_INVALID, "turned dims (%d) must be a multiple of 2 * axes within the head dim (%d)",
+                    r->turned, dim);
+    if (r->turned && !turns) return fail(NATTEN_ERR_INVALID, "NULL operand");
+    return NATTEN_OK;
+}
+
+int check_paged(const natten_paged_t* p) {
+    if (!p) return fail(NATTEN_ERR_INVALID, "problem is NULL");
+    if (p->dtype < NATTEN_F32 || p->dtype > NATTEN_BF16) return fail(NATTEN_ERR_INVALID, "bad dtype %d", p->dtype);
+    if (p->batch < 1 || p->tokens < 1 || p->heads_kv < 1 || p->heads_q < 0)
+        return fail(NATTEN_ERR_INVALID, "batch, tokens and heads must be >= 1");
+    if (p->dim_qk < 1 || p->dim_v < 1) return fail(NATTEN_ERR_INVALID, "head dims must be >= 1");
+    if (p->dim_qk > 256 || p->dim_v > 256)
+        return fail(NATTEN_ERR_UNSUPPORTED, "head dims above 256 are not supported (got %d, %d)", p->dim_qk, p->dim_v);
+    if (p->pages < 1 || p->page_size < 1 || p->table_width < 1)
+        return fail(NATTEN_ERR_INVALID, "pages, page_size and table_width must be >= 1");
+    if (p->table_stride < 0) return fail(NATTEN_ERR_INVALID, "negative table stride");
+    for (int i = 0; i < 3; ++i)
+        if (p->key_stride[i] < 0 || p->value_stride[i] < 0) return fail(NATTEN_ERR_INVALID, "negative page stride");
+    if (static_cast<long long>(p->batch) * p->tokens * (p->heads_q > 0 ? p->heads_q : 1) > (1ll << 30))
+        return fail(NATTEN_ERR_UNSUPPORTED, "batch x tokens x heads above 2^30");
+    return NATTEN_OK;
+}
+
+na::PagedCache to_cache(const natten_paged_t* p, const void* k, const void* v, const int32_t* table,
+                        const int32_t* lens, const int32_t* news) {
+    na::PagedCache c{};
+    c.k = k;
+    c.v = v;
+    for (int i = 0; i < 3; ++i) {
+        c.ks[i] = p->key_stride[i];
+        c.vs[i] = p->value_stride[i];
+    }
+    c.table = table;
+    c.table_stride = p->table_stride;
+    c.lens = lens;
+    c.news = news;
+    c.width = p->table_width;
+    c.pages = p->pages;
+    c.page_size = p->page_size;
+    c.dim_v = p->dim_v;
+    return c;
+}
+
+natten_layout_t page_layout(const int64_t (&st)[3]) { return natten_layout_t{st[0], {0, 0, st[1]}, st[2]}; }
+
+// The attention's problem, checked; pointers and layouts are the caller's.
+int make_paged(const natten_paged_t* p, na::PagedCall& c) {
+    int rc = check_paged(p);
+    if (rc) return rc;
+    if (p->heads_q < 1) return fail(NATTEN_ERR_INVALID, "batch, tokens and heads must be >= 1");
+    if (p->heads_q % p->heads_kv != 0)
+        return fail(NATTEN_ERR_INVALID, "heads_q (%d) must be divisible by heads_kv (%d)", p->heads_q, p->heads_kv);
+    if (p->kernel < 0 || p->dilation < 1) return fail(NATTEN_ERR_INVALID, "kernel and dilation must be >= 1");
+    if (!p->kernel && p->dilation != 1) return fail(NATTEN_ERR_INVALID, "a dilation needs a kernel");
+    c.batch = p->batch;
+    c.tokens = p->tokens;
+    c.heads_q = p->heads_q;
+    c.heads_kv = p->heads_kv;
+    c.dim_qk = p->dim_qk;
+    c.cache.dim_v = p->dim_v;
+    c.cache.width = p->table_width;
+    c.cache.page_size = p->page_size;
+    c.dtype = p->dtype;
+    c.kernel = p->kernel;
+    c.dilation = p->dilation;
+    c.scale = p->scale;
+    return NATTEN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int natten_hip_rotary(const natten_rotary_t* r, const uint64_t* turns, const void* positions, const void* q,
+                      const natten_layout_t* lq, void* q_out, const natten_layout_t* lqo, const void* k,
+                      const natten_layout_t* lk, void* k_out, const natten_layout_t* lko, void* stream) {
+    if (!r) return fail(NATTEN_ERR_INVALID, "problem is NULL");
+    if (r->dtype < NATTEN_F32 || r->dtype > NATTEN_BF16) return fail(NATTEN_ERR_INVALID, "bad dtype %d", r->dtype);
+    if (r->batch < 1 || r->length[0] < 1 || r->length[1] < 1 || r->length[2] < 1)
+        return fail(NATTEN_ERR_INVALID, "batch and lengths must be >= 1");
+    if (r->heads_q < 0 || r->heads_k < 0 || r->heads_q + static_cast<long long>(r->heads_k) < 1)
+        return fail(NATTEN_ERR_INVALID, "heads must be >= 1");
+    if (r->dim < 1) return fail(NATTEN_ERR_INVALID, "head dims must be >= 1");
+    if (r->dim > 256) return fail(NATTEN_ERR_UNSUPPORTED, "head dims above 256 are not supported (got %d)", r->dim);
+    int rc = check_turn(r, r->dim, turns);
+    if (rc) return rc;
+    if (r->position_bits != 0 && r->position_bits != 32 && r->position_bits != 64)
+        return fail(NATTEN_ERR_INVALID, "position_bits must be 0, 32 or 64, got %d", r->position_bits);
+    if (r->position_bits && !positions) return fail(NATTEN_ERR_INVALID, "NULL operand");
+    if (r->heads_q && any_null({q, lq, q_out, lqo})) return fail(NATTEN_ERR_INVALID, "NULL operand");
+    if (r->heads_k && any_null({k, lk, k_out, lko})) return fail(NATTEN_ERR_INVALID, "NULL operand");
+    const long long area = static_cast<long long>(r->length[1]) * r->length[2];
+    if (area > (1ll << 30) || area * r->length[0] > (1ll << 30) || area * r->length[0] * r->batch > (1ll << 30) ||
+        r->heads_q + static_cast<long long>(r->heads_k) > (1 << 16))
+        return fail(NATTEN_ERR_UNSUPPORTED, "more than 2^30 tokens or 2^16 heads");
+    na::RotaryCall c{};
+    c.q = q;
+    c.k = k;
+    c.qo = q_out;
+    c.ko = k_out;
+    c.lq = to_lay(lq);
+    c.lk = to_lay(lk);
+    c.lqo = to_lay(lqo);
+    c.lko = to_lay(lko);
+    c.turns = turns;
+    c.pos = positions;
+    c.pos_bits = r->position_bits;
+    for (int i = 0; i < 3; ++i) {
+        c.pos_stride[i] = r->position_stride[i];
+        c.len[i] = r->length[i];
+    }
+    c.batch = r->batch;
+    c.heads_q = r->heads_q;
+    c.heads_k = r->heads_k;
+    c.dim = r->dim;
+    c.dtype = r->dtype;
+    c.axes = r->axes;
+    c.turned = r->turned;
+    c.interleaved = r->interleaved ? 1 : 0;
+    c.inverse = r->inverse ? 1 : 0;
+    c.magnitude = r->magnitude;
+    c.vec = rotary_vec(r->dtype, r->dim, r->turned, r->axes, 0,
+                       {{r->heads_q ? q : nullptr, lq, r->dim}, {r->heads_q ? q_out : nullptr, lqo, r->dim},
+                        {r->heads_k ? k : nullptr, lk, r->dim}, {r->heads_k ? k_out : nullptr, lko, r->dim}});
+    return launch_status(na::rotary(c, static_cast<hipStream_t>(stream)), "rotary");
+}
+
+int natten_hip_paged_append(const natten_paged_t* p, const natten_rotary_t* r, const uint64_t* turns,
+                            const int32_t* table, const int32_t* seq_lens, const int32_t* new_lens, const void* k,
+                            const natten_layout_t* lk, const void* v, const natten_layout_t* lv, const void* q,
+                            const natten_layout_t* lq, void* q_out, const natten_layout_t* lqo, void* key_pages,
+                            void* value_pages, void* stream) {
+    int rc = check_paged(p);
+    if (rc) return rc;
+    if (any_null({table, seq_lens, k, lk, v, lv, key_pages, value_pages}))
+        return fail(NATTEN_ERR_INVALID, "NULL operand");
+    if (q && (any_null({lq, q_out, lqo}) || p->heads_q < 1)) return fail(NATTEN_ERR_INVALID, "NULL operand");
+    if (p->heads_q + static_cast<long long>(p->heads_kv) > (1 << 16))
+        return fail(NATTEN_ERR_UNSUPPORTED, "more than 2^16 heads");
+    na::RotaryCall c{};
+    c.axes = 1;
+    c.magnitude = 1.f;
+    if (r) {
+        if (r->axes != 1) return fail(NATTEN_ERR_INVALID, "a cache has one axis of positions, got %d", r->axes);
+        rc = check_turn(r, p->dim_qk, turns);
+        if (rc) return rc;
+        c.turned = r->turned;
+        c.interleaved = r->interleaved ? 1 : 0;
+        c.magnitude = r->magnitude;
+        c.turns = turns;
+    }
+    const natten_layout_t lkp = page_layout(p->key_stride), lvp = page_layout(p->value_stride);
+    c.q = q;
+    c.k = k;
+    c.qo = q_out;
+    c.lq = to_lay(q ? lq : nullptr);
+    c.lqo = to_lay(q ? lqo : nullptr);
+    c.lk = to_lay(lk);
+    c.batch = p->batch;
+    c.len[0] = c.len[1] = 1;
+    c.len[2] = p->tokens;
+    c.heads_q = q ? p->heads_q : 0;
+    c.heads_k = p->heads_kv;
+    c.dim = p->dim_qk;
+    c.dtype = p->dtype;
+    c.vec = rotary_vec(p->dtype, p->dim_qk, c.turned, 1, p->dim_v,
+                       {{q, lq, p->dim_qk}, {q ? q_out : nullptr, lqo, p->dim_qk}, {k, lk, p->dim_qk},
+                        {v, lv, p->dim_v}, {key_pages, &lkp, p->dim_qk}, {value_pages, &lvp, p->dim_v}});
+    return launch_status(na::paged_append(to_cache(p, key_pages, value_pages, table, seq_lens, new_lens), c, v,
+                                          to_lay(lv), static_cast<hipStream_t>(stream)),
+                         "paged_append");
+}
+
+int64_t natten_hip_paged_workspace(const natten_paged_t* p) {
+    na::PagedCall c{};
+    if (make_paged(p, c)) return -1;
+    return static_cast<int64_t>(na::paged_workspace(c));
+}
+
+int natten_hip_paged_forward(const natten_paged_t* p, const int32_t* table, const int32_t* seq_lens,
+                             const int32_t* new_lens, const void* q, const natten_layout_t* lq, const void* key_pages,
+                             const void* value_pages, void* out, const natten_layout_t* lo, float* lse,
+                             const natten_layout_t* llse, void* work, int64_t work_bytes, void* stream) {
+    na::PagedCall c{};
+    int rc = make_paged(p, c);
+    if (rc) return rc;
+    if (any_null({table, seq_lens, q, lq, key_pages, value_pages, out, lo, lse, llse}))
+        return fail(NATTEN_ERR_INVALID, "NULL operand");
+    const int64_t need = static_cast<int64_t>(na::paged_workspace(c));
+    if (need && (!work || work_bytes < need || reinterpret_cast<uintptr_t>(work) % 16))
+        return fail(NATTEN_ERR_INVALID, "paged_forward: the workspace must be 16-byte aligned and hold %lld bytes",
+                    static_cast<long long>(need));
+    const natten_layout_t lkp = page_layout(p->key_stride), lvp = page_layout(p->value_stride);
+    c.cache = to_cache(p, key_pages, value_pages, table, seq_lens, new_lens);
+    c.q = q;
+    c.out = out;
+    c.lse = lse;
+    c.lq = to_lay(lq);
+    c.lo = to_lay(lo);
+    c.ll = to_lay(llse);
+    c.work = work;
+    c.vec = runs_aligned(16 / elem_size(p->dtype), {{q, lq, p->dim_qk}, {key_pages, &lkp, p->dim_qk},
+                                                    {value_pages, &lvp, p->dim_v}, {out, lo, p->dim_v}});
+    return launch_status(na::paged_forward(c, static_cast<hipStream_t>(stream)), "paged_forward");
+}
+
+}  // extern "C"

@@ -50,6 +50,53 @@ hipError_t rpb_av_backward(const Prob& p, const void* dout, Lay ldo, const void*
                            void* da, Lay lda, void* dv, Lay ldv, int dtype, hipStream_t s,
                            int sides = kQuerySide | kKeySide);
 
+// Rotary positions (na_rotary.hip) of q (heads_q may be 0) and k (heads_k may
+// be 0) over a grid of tokens.  `turns`: per pair of one axis, turns per
+// position as a 64-bit fraction.  `vec`: elements of an aligned vector that
+// divides an axis's pairs and the dims that do not turn.
+struct RotaryCall {
+    const void *q, *k;
+    void *qo, *ko;
+    Lay lq, lk, lqo, lko;
+    const uint64_t* turns;
+    const void* pos;      // explicit positions, or null: the grid's own
+    int pos_bits;         // 0, 32, 64
+    long long pos_stride[3];  // batch, token, axis
+    int batch, len[3], heads_q, heads_k, dim, dtype, vec;
+    int axes, turned, interleaved, inverse;
+    float magnitude;
+};
+hipError_t rotary(const RotaryCall& c, hipStream_t s);
+
+// Pages of keys and values [pages, page_size, Hkv, D] at their strides (page,
+// slot, head), the pages of each sequence, its tokens and how many are new.
+struct PagedCache {
+    const void *k, *v;
+    long long ks[3], vs[3];
+    const int* table;
+    long long table_stride;
+    const int *lens, *news;  // news null: all tokens of the call
+    int width, pages, page_size, dim_v;
+};
+// The new tokens' keys (turned, as r says) and values v into their pages; r.q
+// turned into r.qo, zeros at padding (r.ko and r.lko are not used).
+hipError_t paged_append(const PagedCache& c, const RotaryCall& r, const void* v, Lay lv, hipStream_t s);
+
+// Attention of the new tokens over the cache (na_paged.hip).
+struct PagedCall {
+    PagedCache cache;
+    const void* q;
+    void* out;
+    float* lse;
+    Lay lq, lo, ll;
+    int batch, tokens, heads_q, heads_kv, dim_qk, dtype;
+    int kernel, dilation;  // kernel 0: every key up to the query's own
+    float scale;
+    bool vec;    // 16-byte aligned q, out and pages, head dims a multiple of a vector
+    void* work;  // paged_workspace bytes
+};
+size_t paged_workspace(const PagedCall& c);
+hipError_t paged_forward(const PagedCall& c, hipStream_t s);
 
 }  // namespace na
 

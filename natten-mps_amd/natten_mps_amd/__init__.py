@@ -24,6 +24,12 @@ __all__ = [
     "na3d_qk",
     "na3d_av",
     "merge_attentions",
+    "RotaryPlan",
+    "rotary",
+    "rotary_qk",
+    "PagedKVCache",
+    "na1d_paged",
+    "na1d_paged_append",
     "NeighborhoodAttention1D",
     "NeighborhoodAttention2D",
     "NeighborhoodAttention3D",
@@ -40,6 +46,8 @@ _LAZY_ATTRS = {
         "na1d", "na1d_varlen", "na1d_qk", "na1d_av", "na2d", "na2d_varlen", "na2d_qk", "na2d_av",
         "na3d", "na3d_varlen", "na3d_qk", "na3d_av")},
     "merge_attentions": "natten_mps_amd.merge",
+    **{n: "natten_mps_amd.positions" for n in ("RotaryPlan", "rotary", "rotary_qk")},
+    **{n: "natten_mps_amd.paged" for n in ("PagedKVCache", "na1d_paged", "na1d_paged_append")},
     "NeighborhoodAttention1D": "natten_mps_amd.nn",
     "NeighborhoodAttention2D": "natten_mps_amd.nn",
     "NeighborhoodAttention3D": "natten_mps_amd.nn",

@@ -49,6 +49,10 @@ ENTRY_POINTS = (
     "natten_hip_rpb_dbias_workspace",
     "natten_hip_rpb_qk_backward_ws",
     "natten_hip_rpb_av_backward",
+    "natten_hip_rotary",
+    "natten_hip_paged_append",
+    "natten_hip_paged_workspace",
+    "natten_hip_paged_forward",
     "natten_hip_profile_enable",
     "natten_hip_profile_read",
 )
@@ -71,6 +75,21 @@ class Problem(ctypes.Structure):
         ("stride", ctypes.c_int32 * 3),
         ("causal", ctypes.c_int32 * 3),
     ]
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [(n, t) for n, t in (
+        ("batch", ctypes.c_int32), ("length", ctypes.c_int32 * 3), ("heads_q", ctypes.c_int32),
+        ("heads_k", ctypes.c_int32), ("dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("axes", ctypes.c_int32),
+        ("turned", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("magnitude", ctypes.c_float), ("position_bits", ctypes.c_int32), ("position_stride", ctypes.c_int64 * 3))]
+
+
+class Paged(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "batch", "tokens", "heads_q", "heads_kv", "dim_qk", "dim_v", "dtype", "pages", "page_size", "table_width")] + [
+        ("table_stride", ctypes.c_int64), ("key_stride", ctypes.c_int64 * 3), ("value_stride", ctypes.c_int64 * 3),
+        ("kernel", ctypes.c_int32), ("dilation", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
 class KernelStat(ctypes.Structure):
@@ -114,6 +133,11 @@ _SIGNATURES = {
     "natten_hip_rpb_qk_backward_ws": ([_P(Problem)] + [_VP, _LP] * 5 + [_VP, _VP, ctypes.c_int64, _VP],
                                       ctypes.c_int),
     "natten_hip_rpb_av_backward": ([_P(Problem)] + [_VP, _LP] * 5 + [_VP], ctypes.c_int),
+    "natten_hip_rotary": ([_P(Rotary), _VP, _VP] + [_VP, _LP] * 4 + [_VP], ctypes.c_int),
+    "natten_hip_paged_append": ([_P(Paged), _P(Rotary)] + [_VP] * 4 + [_VP, _LP] * 4 + [_VP] * 3, ctypes.c_int),
+    "natten_hip_paged_workspace": ([_P(Paged)], ctypes.c_int64),
+    "natten_hip_paged_forward": ([_P(Paged)] + [_VP] * 3 + [_VP, _LP, _VP, _VP] + [_VP, _LP] * 2
+                                 + [_VP, ctypes.c_int64, _VP], ctypes.c_int),
     "natten_hip_profile_enable": ([ctypes.c_int], ctypes.c_int),
     "natten_hip_profile_read": ([_P(KernelStat), ctypes.c_int, ctypes.c_int], ctypes.c_int),
 }

@@ -914,3 +914,134 @@ def _bind(rank: int) -> None:
 for _r in (1, 2, 3):
     _bind(_r)
 del _r
+
+
+# ---------------------------------------------------------------------------
+# rotary positions and the paged cache
+# ---------------------------------------------------------------------------
+
+
+def _int32(t: Optional[torch.Tensor], device) -> Optional[torch.Tensor]:
+    """Lengths and page numbers as the kernels read them; int64 values past
+    int32 stay out of range."""
+    if t is None or t.dtype == torch.int32:
+        return t
+    return t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+
+
+def _axis_lay(t: torch.Tensor) -> "_lib.Layout":
+    return _lib.layout(t, t.ndim - 3, 1)
+
+
+def rotary(q, k, plan, positions, inverse):
+    """``(q', k')``: q and k (None: absent) turned by their positions."""
+    _on_device(q, k, positions)
+    _same_dtype(q, k)
+    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        return outs
+    q = _inner(q)
+    k = None if k is None else _inner(k)
+    # a tensor without heads beside one with some is absent
+    tq, tk = (None if t is None or t.numel() == 0 else t for t in (q, k))
+    rank = q.ndim - 3
+    r = _lib.Rotary()
+    r.batch, r.dim, r.dtype = q.shape[0], q.shape[-1], _lib.dtype_code(q)
+    r.length[:] = [1] * (3 - rank) + list(q.shape[1:1 + rank])
+    r.heads_q = 0 if tq is None else tq.shape[-2]
+    r.heads_k = 0 if tk is None else tk.shape[-2]
+    r.axes, r.turned, r.magnitude = plan.axes, plan.dim, plan.magnitude
+    r.interleaved, r.inverse = int(plan.interleaved), int(inverse)
+    if positions is not None:
+        lead = positions.ndim - (0 if plan.axes == 1 else 1)
+        pos = positions.contiguous()
+        n = pos.numel() // (pos.shape[0] if lead == rank + 1 else 1)
+        r.position_bits = 32 if pos.dtype == torch.int32 else 64
+        r.position_stride[:] = [n if lead == rank + 1 and pos.shape[0] > 1 else 0, plan.axes, 1]
+    else:
+        pos = None
+    args = []
+    for t, o in ((tq, outs[0]), (tk, outs[1])):
+        args += [None, None, None, None] if t is None else [
+            t.data_ptr(), _byref(_axis_lay(t)), o.data_ptr(), _byref(_axis_lay(o))]
+    rc = _launch(q.device, _lib.load().natten_hip_rotary, _byref(r), plan.table(q.device).data_ptr(),
+                 None if pos is None else pos.data_ptr(), *args, _raw_stream(q.device))
+    _lib.check(rc, "rotary")
+    return outs
+
+
+def _paged_problem(batch, tokens, heads_q, key_pages, value_pages, table):
+    p = _lib.Paged()
+    p.batch, p.tokens, p.heads_q = batch, tokens, heads_q
+    p.pages, p.page_size, p.heads_kv, p.dim_qk = key_pages.shape
+    p.dim_v = value_pages.shape[-1]
+    p.dtype = _lib.dtype_code(key_pages)
+    p.table_width, p.table_stride = table.shape[1], table.stride(0)
+    p.key_stride[:] = key_pages.stride()[:3]
+    p.value_stride[:] = value_pages.stride()[:3]
+    p.dilation = 1
+    return p
+
+
+def _table_rows(table: torch.Tensor) -> torch.Tensor:
+    return table if table.stride(1) == 1 else table.contiguous()
+
+
+def paged_append(key, value, key_pages, value_pages, table, seq_lens, new_lens, query, plan):
+    """Turned keys and values into their pages; the turned query or None."""
+    _on_device(key, value, key_pages, value_pages, table, seq_lens, new_lens, query)
+    _same_dtype(key, value, key_pages, value_pages, query)
+    out = None if query is None else torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if key.numel() == 0:
+        return out
+    dev = key.device
+    key, value = _inner(key), _inner(value)
+    query = None if query is None or query.numel() == 0 else _inner(query)
+    table = _table_rows(_int32(table, dev))
+    lens, news = _int32(seq_lens, dev).contiguous(), _int32(new_lens, dev)
+    news = None if news is None else news.contiguous()
+    p = _paged_problem(key.shape[0], key.shape[1], 0 if query is None else query.shape[2], key_pages, value_pages,
+                       table)
+    r = turns = None
+    if plan is not None:
+        r = _lib.Rotary()
+        r.axes, r.turned, r.magnitude, r.interleaved = 1, plan.dim, plan.magnitude, int(plan.interleaved)
+        turns = plan.table(dev).data_ptr()
+    qargs = [None] * 4 if query is None else [query.data_ptr(), _byref(_axis_lay(query)), out.data_ptr(),
+                                              _byref(_axis_lay(out))]
+    rc = _launch(dev, _lib.load().natten_hip_paged_append, _byref(p), None if r is None else _byref(r), turns,
+                 table.data_ptr(), lens.data_ptr(), None if news is None else news.data_ptr(),
+                 key.data_ptr(), _byref(_axis_lay(key)), value.data_ptr(), _byref(_axis_lay(value)), *qargs,
+                 key_pages.data_ptr(), value_pages.data_ptr(), _raw_stream(dev))
+    _lib.check(rc, "paged_append")
+    return out
+
+
+def paged_forward(query, key_pages, value_pages, table, seq_lens, new_lens, kernel_size, dilation, scale):
+    """``(out, lse)`` of the new tokens' queries; lse is fp32 ``[B, L, Hq]``."""
+    _on_device(query, key_pages, value_pages, table, seq_lens, new_lens)
+    _same_dtype(query, key_pages, value_pages)
+    dev = query.device
+    B, L, Hq, _ = query.shape
+    out = torch.empty((B, L, Hq, value_pages.shape[-1]), dtype=query.dtype, device=dev)
+    lse = torch.empty((B, L, Hq), dtype=torch.float32, device=dev)
+    if B == 0 or L == 0:
+        return out, lse
+    query = _inner(query)
+    table = _table_rows(_int32(table, dev))
+    lens, news = _int32(seq_lens, dev).contiguous(), _int32(new_lens, dev)
+    news = None if news is None else news.contiguous()
+    p = _paged_problem(B, L, Hq, key_pages, value_pages, table)
+    p.kernel = 0 if kernel_size is None else min(kernel_size, 2 ** 31 - 1)
+    p.dilation = min(dilation, 2 ** 31 - 1)
+    p.scale = scale
+    lib = _lib.load()
+    need = max(lib.natten_hip_paged_workspace(_byref(p)), 0)  # below 0: the call itself reports the problem
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rc = _launch(dev, lib.natten_hip_paged_forward, _byref(p), table.data_ptr(), lens.data_ptr(),
+                 None if news is None else news.data_ptr(), query.data_ptr(), _byref(_axis_lay(query)),
+                 key_pages.data_ptr(), value_pages.data_ptr(), out.data_ptr(), _byref(_axis_lay(out)),
+                 lse.data_ptr(), _byref(_lib.layout(lse, 1, 0)), None if work is None else work.data_ptr(), need,
+                 _raw_stream(dev))
+    _lib.check(rc, "paged_forward")
+    return out, lse

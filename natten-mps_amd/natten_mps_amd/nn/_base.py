@@ -13,6 +13,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from natten_mps_amd import functional as F
+from natten_mps_amd.positions import RotaryPlan, check_plan, rotary_qk
 from natten_mps_amd.utils.params import normalize_tuple_param
 
 _SHAPES = {1: "[B, L, C]", 2: "[B, H, W, C]", 3: "[B, D, H, W, C]"}
@@ -25,7 +26,7 @@ class _NeighborhoodAttentionND(torch.nn.Module):
                  stride: Union[int, Tuple[int, ...]] = 1, dilation: Union[int, Tuple[int, ...]] = 1,
                  is_causal: Union[bool, Tuple[bool, ...]] = False, num_kv_heads: Optional[int] = None,
                  qkv_bias: bool = True, qk_scale: Optional[float] = None, attn_drop: float = 0.0,
-                 proj_drop: float = 0.0):
+                 proj_drop: float = 0.0, rotary: Optional[RotaryPlan] = None):
         super().__init__()
         r = self.rank
         if embed_dim % num_heads != 0:
@@ -53,8 +54,13 @@ class _NeighborhoodAttentionND(torch.nn.Module):
         self.attn_drop = torch.nn.Dropout(attn_drop)
         self.proj = torch.nn.Linear(self.embed_dim, self.embed_dim)
         self.proj_drop = torch.nn.Dropout(proj_drop)
+        if rotary is not None:
+            check_plan(rotary, self.head_dim)
+            if rotary.axes != r:
+                raise ValueError(f"the rotary plan has {rotary.axes} axes, the module {r}.")
+        self.rotary = rotary
 
-    def forward(self, x, sizes=None):
+    def forward(self, x, sizes=None, cache=None):
         r = self.rank
         if x.ndim != r + 2:
             raise ValueError(f"NeighborhoodAttention{r}D expects input shape {_SHAPES[r]}.")
@@ -71,6 +77,11 @@ class _NeighborhoodAttentionND(torch.nn.Module):
             qkv = self.qkv(x).reshape(bsz, *sp, 3, self.num_heads, self.head_dim).permute(*perm)
             q, k, v = qkv.unbind(0)
 
+        if cache is not None:
+            out = self._attend_cached(q, k, v, cache)
+            return self.proj_drop(self.proj(out.reshape(bsz, *sp, self.embed_dim)))
+        if self.rotary is not None:
+            q, k = rotary_qk(q, k, self.rotary)
         if sizes is not None:
             out = getattr(F, f"na{r}d_varlen")(q, k, v, sizes, kernel_size=self.kernel_size,
                                                dilation=self.dilation, scale=self.scale)
