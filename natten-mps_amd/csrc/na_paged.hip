@@ -137,6 +137,267 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_rows(PagedArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// 16-bit types on MFMA
+// ---------------------------------------------------------------------------
+
+// Elements of an LDS row of head dim D, and the swizzle of its 16-byte pieces:
+// the 16 rows x 32 bytes of a transposing read, and the rows that 8 lanes
+// write, lie on distinct banks.
+template <int D>
+constexpr int row_elems() {
+    return D == 96 ? 128 : D;
+}
+
+template <int D>
+__device__ __forceinline__ int piece_swz(int row) {
+    constexpr int LD = row_elems<D>();
+    const int odd = (row >> 3) & 1;
+    if constexpr (LD == 128) return ((row & 7) << 1) | odd;
+    else if constexpr (LD == 64) return (((row >> 1) & 3) << 1) | odd;
+    else return (((row >> 2) & 1) << 1) | odd;
+}
+
+// The scale's sign goes into the queries (exact), a scale of zero makes them
+// zero, so that scores times `sc2` > 0 order as the logits do.
+struct ScaleParts {
+    float sc2;
+    uint32_t flip, keep;  // of two 16-bit elements
+};
+
+__device__ __forceinline__ ScaleParts scale_parts(float scale) {
+    ScaleParts r;
+    r.sc2 = scale == 0.f ? 1.f : __builtin_fabsf(scale) * kLog2e;
+    r.flip = scale < 0.f ? 0x80008000u : 0u;
+    r.keep = scale == 0.f ? 0u : 0xffffffffu;
+    return r;
+}
+
+__device__ __forceinline__ uint4 scaled(uint4 x, const ScaleParts& s) {
+    return make_uint4((x.x & s.keep) ^ s.flip, (x.y & s.keep) ^ s.flip, (x.z & s.keep) ^ s.flip,
+                      (x.w & s.keep) ^ s.flip);
+}
+
+// One key's part of a row's products, in plain arithmetic: acc[e] += p v[dv]
+// for `N` runs of four head dims from dv0 in steps of `step`.  Keys and pages
+// that the row does not attend to are not touched.
+template <typename T, int D, int N, int STEP>
+__device__ __forceinline__ void exact_key(const PagedArgs& a, const Share& r, const int* table, const T* q, int u,
+                                          int lo, int hi, float m, int dv0, f32x4_t (&acc)[N]) {
+    int page, slot;
+    if (u < lo || u > hi || !key_at(a, table, r.c, u, r.u_hi, page, slot)) return;
+    const T* const k = static_cast<const T*>(a.k) + (page * a.kp + slot * a.ks + r.h * a.kh);
+    const T* const v = static_cast<const T*>(a.v) + (page * a.vp + slot * a.vs + r.h * a.vh) + dv0;
+    float dot = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < D; ++d) dot = fmaf(to_f(q[d]), to_f(k[d]), dot);
+    const float p = __builtin_amdgcn_exp2f(dot * (a.scale * kLog2e) - m);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(p, to_f(v[n * STEP + i]), acc[n][i]);
+}
+
+// 16 rows, the four waves on different keys, 32 at a time each.
+//
+// Scores as S^T = K Q^T (v_mfma 16x16x32): a lane then holds one query (its
+// column) and keys 4g..4g+3 of each 16-key block (g its 16-lane row), so the
+// softmax of a query is in-lane but for two lane exchanges, and the packed
+// probabilities are at once the B operand of O^T = V^T P^T, whose k slots are
+// those keys.  K goes straight from the pages to registers in the A layout
+// (lane: key `col`, 16-byte pieces g, g + 4, ..); V, read the same way, is
+// written to the wave's own LDS and read back transposed.
+//
+// Each key is read once per kv head and nothing else is big, so HBM bounds
+// it: the next keys' loads are issued as soon as the registers are free, and
+// page numbers one step before that.
+constexpr int kFewRows = 16, kFewKeys = 32;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
+    constexpr int C = D / 32, LD = row_elems<D>(), DB = D / 16;
+    __shared__ ShareScratch sh;
+    __shared__ __attribute__((aligned(16))) T vs[4][kFewKeys * LD];
+    __shared__ float ml[4][kFewRows][2];
+    clear_padding<T>(a);
+    Share r;
+    if (!find_share(a, sh, r)) return;
+    if (r.rows <= 0) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int col = lane & 15, g = lane >> 4;
+    const int row = r.row0 + imin(col, r.rows - 1);
+    int qi, qh;
+    row_token(a, r.cls, r.h, row, qi, qh);
+    const T* const q = static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
+    const ScaleParts sp = scale_parts(a.scale);
+    uint4 qf[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) qf[c] = scaled(*reinterpret_cast<const uint4*>(q + 32 * c + 8 * g), sp);
+    // the row's window, and what all rows of the tile see
+    const int hi = r.w0 + fdiv(row, a.frep), lo = a.K ? hi - a.K + 1 : 0;
+    const int all_hi = imin(r.w0 + fdiv(r.row0, a.frep), r.u_hi);
+    const int all_lo = a.K ? r.w0 + fdiv(r.row0 + r.rows - 1, a.frep) - a.K + 1 : 0;
+    const int steps = (r.u_hi - r.u_lo + kFewKeys) / kFewKeys;  // 0 when empty: u_hi = u_lo - 1 at least
+    const int* const table = a.table + r.b * a.table_stride;
+    const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh + 8 * g;
+    const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh + 8 * g;
+    T* const X = vs[wave];
+
+    int page[2], slot[2];
+    auto lookup = [&](int st) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int u = imin(r.u_lo + st * kFewKeys + 16 * b + col, r.u_hi);
+            const int j = r.c + u * a.dil;
+            const int pg = fdiv(j, a.fpage);
+            slot[b] = j - pg * a.page_size;
+            page[b] = table[pg];
+        }
+    };
+    uint4 kf[2][C], vf[2][C];
+    bool ok[2];
+    auto load = [&](int st) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            ok[b] = page[b] >= 0 && page[b] < a.pages && r.u_lo + st * kFewKeys + 16 * b + col <= r.u_hi;
+            // keys that are not there: the pool's first slot, masked below
+            const int pg = ok[b] ? page[b] : 0, sl = ok[b] ? slot[b] : 0;
+            const T* const k = kb + (pg * a.kp + sl * a.ks);
+            const T* const v = vb + (pg * a.vp + sl * a.vs);
+#pragma unroll
+            for (int c = 0; c < C; ++c) kf[b][c] = *reinterpret_cast<const uint4*>(k + 32 * c);
+#pragma unroll
+            for (int c = 0; c < C; ++c) vf[b][c] = *reinterpret_cast<const uint4*>(v + 32 * c);
+        }
+    };
+
+    float m = -INFINITY, l = 0.f;
+    f32x4_t o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (wave < steps) {
+        lookup(wave);
+        load(wave);
+        if (wave + 4 < steps) lookup(wave + 4);
+    }
+    for (int st = wave; st < steps; st += 4) {
+        const int ub = r.u_lo + st * kFewKeys;
+        f32x4_t s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            s[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < C; ++c) s[b] = Mma<T>::run(kf[b][c], qf[c], s[b]);
+        }
+        const bool there[2] = {ok[0], ok[1]};
+        const unsigned long long have0 = __ballot(there[0]), have1 = __ballot(there[1]);
+        const bool whole = (have0 & have1) == ~0ull;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int rw = 16 * b + col, sw = piece_swz<D>(rw);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                uint4 x = vf[b][c];
+                if (!whole && !there[b]) x = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(X + rw * LD + (((4 * c + g) ^ sw) << 3)) = x;
+            }
+        }
+        if (st + 4 < steps) {
+            load(st + 4);
+            if (st + 8 < steps) lookup(st + 8);
+        }
+        if (!whole || ub + kFewKeys - 1 > all_hi || ub < all_lo) {
+            const uint32_t bits[2] = {static_cast<uint32_t>(have0 >> (4 * g)), static_cast<uint32_t>(have1 >> (4 * g))};
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int u = ub + 16 * b + 4 * g + i;
+                    if (!((bits[b] >> i) & 1) || u > hi || u < lo) s[b][i] = -INFINITY;
+                }
+        }
+        const float m2 = fmaxp(m, max_rows(max8(s)) * sp.sc2);
+        const float ref = m2 == -INFINITY ? 0.f : m2;
+        if (__ballot(m2 != m)) {
+            const float keep = __builtin_amdgcn_exp2f(m - ref);
+            l *= keep;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[db] *= keep;
+        }
+        m = m2;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], sp.sc2, -ref));
+                l += s[b][i];
+            }
+        const uint4 p = pack8<T>(s);
+        const int r0 = 4 * g + (col >> 2), r1 = 16 + r0;
+        const int s0 = piece_swz<D>(r0), s1 = piece_swz<D>(r1);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            const int pc = 2 * db + ((col & 3) >> 1);
+            const T* const x0 = X + r0 * LD + ((pc ^ s0) << 3) + (col & 1) * 4;
+            const T* const x1 = X + r1 * LD + ((pc ^ s1) << 3) + (col & 1) * 4;
+            const uint2 lo2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x0));
+            const uint2 hi2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x1));
+            o[db] = Mma<T>::run(make_uint4(lo2.x, lo2.y, hi2.x, hi2.y), p, o[db]);
+        }
+    }
+    l = sum_rows(l);
+    // A probability of 0 times a value that is not finite: rows of the tile
+    // that do not attend to that key got NaN.  Redone key by key.
+    if (item_nonfinite(lane_sum(o, 0.f)) && !item_nonfinite(m) && !item_nonfinite(l)) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int st = wave; st < steps; st += 4)
+            for (int e = 0; e < kFewKeys; ++e)
+                exact_key<T, D, DB, 16>(a, r, table, q, r.u_lo + st * kFewKeys + e, lo, hi, m, 4 * g, o);
+    }
+    // the four waves' parts, through the LDS that held their values
+    float* const ow = reinterpret_cast<float*>(X);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+        *reinterpret_cast<f32x4_t*>(ow + col * D + 16 * db + 4 * g) = o[db];
+    if (g == 0) {
+        ml[wave][col][0] = m;
+        ml[wave][col][1] = l;
+    }
+    lds_publish_barrier();
+    for (int e = threadIdx.x; e < kFewRows * (D / 4); e += kPagedThreads) {
+        const int rw = e / (D / 4), d = 4 * (e - rw * (D / 4));
+        if (rw >= r.rows) break;
+        const float mt = fmaxp(fmaxp(ml[0][rw][0], ml[1][rw][0]), fmaxp(ml[2][rw][0], ml[3][rw][0]));
+        const float ref = mt == -INFINITY ? 0.f : mt;
+        float lt = 0.f;
+        f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (ml[w][rw][0] == -INFINITY && ml[w][rw][1] == 0.f) continue;
+            const float wt = __builtin_amdgcn_exp2f(ml[w][rw][0] - ref);
+            lt = fmaf(wt, ml[w][rw][1], lt);
+            x += wt * *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(vs[w]) + rw * D + d);
+        }
+        if (r.split) {
+            const long long at = static_cast<long long>(r.index) * kFewRows + rw;
+            *reinterpret_cast<f32x4_t*>(a.part + at * D + d) = x;
+            if (d == 0) {
+                a.ml[2 * at] = mt;
+                a.ml[2 * at + 1] = lt;
+            }
+            continue;
+        }
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        int i, hq;
+        row_token(a, r.cls, r.h, r.row0 + rw, i, hq);
+        T* const out = static_cast<T*>(a.out) + r.b * a.lo.b + i * a.lo.s2 + hq * a.lo.h + d;
+        *reinterpret_cast<uint2*>(out) = make_uint2(Mma<T>::pack(x[0] * inv, x[1] * inv),
+                                                    Mma<T>::pack(x[2] * inv, x[3] * inv));
+        if (d == 0) a.lse[r.b * a.ll.b + i * a.ll.s2 + hq * a.ll.h] = row_lse(mt, lt);
+    }
+}
+
+// ---------------------------------------------------------------------------
 // joining parts
 // ---------------------------------------------------------------------------
 
@@ -210,7 +471,10 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_join(PagedArgs a) {
 // Workgroups aimed at when the tiles are few: two a compute unit.
 constexpr int kTarget = 512;
 
+enum PagedKind { kRows, kFew };
+
 struct PagedPlan {
+    PagedKind kind;
     int M, KT, least, xcd_run;
     long long tiles;  // tile slots of the batch
     int slots;        // of a (sequence, kv head)
@@ -221,11 +485,25 @@ struct PagedPlan {
 
 long long padded(long long bytes) { return (bytes + 255) & ~255ll; }
 
+// MFMA kernels: 16-bit, equal head dims that they are built for, operands
+// read and written in 16-byte vectors.
+bool on_mfma(const PagedCall& c) {
+    const int d = c.dim_qk;
+    return c.dtype != NATTEN_F32 && c.vec && d == c.cache.dim_v && (d == 32 || d == 64 || d == 96 || d == 128);
+}
+
 PagedPlan plan(const PagedCall& c) {
     PagedPlan p{};
-    p.M = 4;
-    p.KT = 64;
-    p.least = 4;
+    p.kind = on_mfma(c) ? kFew : kRows;
+    if (p.kind == kFew) {
+        p.M = kFewRows;
+        p.KT = 4 * kFewKeys;
+        p.least = 2;
+    } else {
+        p.M = 4;
+        p.KT = 64;
+        p.least = 4;
+    }
     p.xcd_run = 0;
     const long long rep = c.heads_q / c.heads_kv;
     const long long dil = c.dilation, classes = c.tokens < dil ? c.tokens : dil;
@@ -253,13 +531,32 @@ PagedPlan plan(const PagedCall& c) {
 }
 
 template <typename T>
-hipError_t launch_rows(const PagedArgs& a, const PagedPlan& p, bool vec, hipStream_t s) {
-    constexpr int kVec = 16 / sizeof(T);
-    if (vec)
-        NA_LAUNCH("na_paged_rows", (k_paged_rows<T, kVec>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
+hipError_t launch_few(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+    const dim3 grid(p.grid), block(kPagedThreads);
+    if (a.Dqk == 32)
+        NA_LAUNCH("na_paged_few", (k_paged_few<T, 32>), grid, block, 0, s, a);
+    else if (a.Dqk == 64)
+        NA_LAUNCH("na_paged_few", (k_paged_few<T, 64>), grid, block, 0, s, a);
+    else if (a.Dqk == 96)
+        NA_LAUNCH("na_paged_few", (k_paged_few<T, 96>), grid, block, 0, s, a);
     else
-        NA_LAUNCH("na_paged_rows", (k_paged_rows<T, 1>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
-    hipError_t e = hipGetLastError();
+        NA_LAUNCH("na_paged_few", (k_paged_few<T, 128>), grid, block, 0, s, a);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_kind(const PagedArgs& a, const PagedPlan& p, bool vec, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    if (p.kind == kRows) {
+        constexpr int kVec = 16 / sizeof(T);
+        if (vec)
+            NA_LAUNCH("na_paged_rows", (k_paged_rows<T, kVec>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
+        else
+            NA_LAUNCH("na_paged_rows", (k_paged_rows<T, 1>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
+        e = hipGetLastError();
+    } else if constexpr (!std::is_same<T, float>::value) {
+        e = launch_few<T>(a, p, s);
+    }
     if (e != hipSuccess || !p.split) return e;
     NA_LAUNCH("na_paged_join", (k_paged_join<T>), dim3(p.tiles < kTarget ? p.tiles : kTarget, p.M),
               dim3(kPagedThreads), 0, s, a);
@@ -268,7 +565,16 @@ hipError_t launch_rows(const PagedArgs& a, const PagedPlan& p, bool vec, hipStre
 
 }  // namespace
 
-size_t paged_workspace(const PagedCall& c) { return plan(c).bytes; }
+// The most that a call of this problem takes, whatever its operands' alignment.
+size_t paged_workspace(const PagedCall& c) {
+    PagedCall x = c;
+    size_t most = 0;
+    for (bool vec : {false, true}) {
+        x.vec = vec;
+        most = std::max(most, plan(x).bytes);
+    }
+    return most;
+}
 
 hipError_t paged_forward(const PagedCall& c, hipStream_t s) {
     const PagedPlan p = plan(c);
@@ -327,9 +633,9 @@ hipError_t paged_forward(const PagedCall& c, hipStream_t s) {
         w += padded(sizeof(float) * 2 * p.M * 2 * kTarget);
         a.part = reinterpret_cast<float*>(w);
     }
-    if (c.dtype == NATTEN_F32) return launch_rows<float>(a, p, c.vec, s);
-    if (c.dtype == NATTEN_F16) return launch_rows<f16>(a, p, c.vec, s);
-    return launch_rows<bf16>(a, p, c.vec, s);
+    if (c.dtype == NATTEN_F32) return launch_kind<float>(a, p, c.vec, s);
+    if (c.dtype == NATTEN_F16) return launch_kind<f16>(a, p, c.vec, s);
+    return launch_kind<bf16>(a, p, c.vec, s);
 }
 
 }  // namespace na
