@@ -11,6 +11,8 @@
 // k_paged_few   16-bit, head dim 32/64/96/128: 16 rows a workgroup on MFMA,
 //               its four waves on different keys.  The cache is read once, so
 //               HBM bounds it.
+// k_paged_chunk the same types, many rows: 128 or 256 rows a workgroup on
+//               MFMA, keys and values staged in LDS for all its waves.
 // k_paged_join  joins the parts of tiles whose keys were cut.
 #include <type_traits>
 
@@ -398,11 +400,338 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
 }
 
 // ---------------------------------------------------------------------------
+// many rows
+// ---------------------------------------------------------------------------
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <typename T>
+__device__ __forceinline__ f32x16_t mma32(uint4 a, uint4 b, f32x16_t c) {
+    if constexpr (std::is_same<T, bf16>::value)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                      0, 0, 0);
+}
+
+// Swizzles of the chunk kernel's LDS rows (16-byte pieces).  Keys: 16 rows of
+// one piece on distinct banks; values: the 8 rows x 2 pairs of pieces of a
+// transposing read.
+template <int LD>
+__device__ __forceinline__ int key_swz(int row) {
+    if constexpr (LD == 128) return row & 15;
+    else if constexpr (LD == 64) return (row >> 1) & 7;
+    else return (row >> 2) & 3;
+}
+
+template <int LD>
+__device__ __forceinline__ int value_swz(int row) {
+    if constexpr (LD == 128) return (row & 7) << 1;
+    else if constexpr (LD == 64) return ((row >> 1) & 3) << 1;
+    else return ((row >> 2) & 1) << 1;
+}
+
+// The other half-wave's value of the same query.
+__device__ __forceinline__ float other_half(float v) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? x[0] : x[1]);
+}
+
+// 128 QB rows a workgroup: a wave has 32 QB queries (columns of 32x32x16
+// products), all waves the same 64 keys, staged in LDS twice over.  As in
+// k_paged_few, scores are K Q^T and results V^T P^T, so that the packed
+// probabilities are the second product's operand as they lie: of the 16
+// accumulators of a 32-key block, half-wave h holds keys 8 (i / 4) + 4 h +
+// i % 4, and the values' operand is read (transposed) in that order.
+constexpr int kChunkKeys = 64;
+
+template <typename T, int D, int QB>
+__global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
+    constexpr int C = D / 16, LD = row_elems<D>(), DT = D / 32;
+    constexpr int PR = D / 8;                        // pieces of a row
+    constexpr int kLoads = kChunkKeys * PR / kPagedThreads;  // of a thread, keys and values each
+    constexpr int kTile = kChunkKeys * LD;
+    __shared__ ShareScratch sh;
+    __shared__ long long koff[2][kChunkKeys], voff[2][kChunkKeys];
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    T* const ks = reinterpret_cast<T*>(lds);
+    T* const vs = ks + 2 * kTile;
+    clear_padding<T>(a);
+    Share r;
+    if (!find_share(a, sh, r)) return;
+    if (r.rows <= 0) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int col = lane & 31, h = lane >> 5;
+    const ScaleParts sp = scale_parts(a.scale);
+    const int* const table = a.table + r.b * a.table_stride;
+    const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh;
+    const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh;
+    const int wrow = 32 * QB * wave;  // the wave's first row in the tile
+    uint4 qf[QB][C];
+    int hi[QB], lo[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const int row = r.row0 + imin(wrow + 32 * b + col, r.rows - 1);
+        int qi, qh;
+        row_token(a, r.cls, r.h, row, qi, qh);
+        const T* const q = static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
+#pragma unroll
+        for (int c = 0; c < C; ++c) qf[b][c] = scaled(*reinterpret_cast<const uint4*>(q + 16 * c + 8 * h), sp);
+        hi[b] = r.w0 + fdiv(row, a.frep);
+        lo[b] = a.K ? hi[b] - a.K + 1 : 0;
+    }
+    // what some and what all rows of the wave see
+    const int wf = r.w0 + fdiv(r.row0 + imin(wrow, r.rows - 1), a.frep);
+    const int wl = r.w0 + fdiv(r.row0 + imin(wrow + 32 * QB, r.rows) - 1, a.frep);
+    const int some_lo = a.K ? wf - a.K + 1 : 0, all_lo = a.K ? wl - a.K + 1 : 0;
+    const bool idle = wrow >= r.rows;
+    const int steps = (r.u_hi - r.u_lo + kChunkKeys) / kChunkKeys;
+
+    // Offsets of tile st's keys by lane, -1 where no page holds one; the page
+    // number is asked for well before.
+    int page = -1, slot = 0;
+    auto ask = [&](int st) {
+        if (!key_at(a, table, r.c, r.u_lo + st * kChunkKeys + lane, r.u_hi, page, slot)) page = -1;
+    };
+    auto locate = [&](int st) {
+        koff[st & 1][lane] = page >= 0 ? page * a.kp + slot * a.ks : -1;
+        voff[st & 1][lane] = page >= 0 ? page * a.vp + slot * a.vs : -1;
+    };
+    uint4 kx[kLoads], vx[kLoads];
+    auto load = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int rw = (tid + i * kPagedThreads) / PR, lpc = (tid + i * kPagedThreads) % PR;
+            const long long ko = koff[st & 1][rw], vo = voff[st & 1][rw];
+            kx[i] = make_uint4(0, 0, 0, 0);
+            vx[i] = make_uint4(0, 0, 0, 0);
+            if (ko >= 0) {
+                kx[i] = *reinterpret_cast<const uint4*>(kb + ko + 8 * lpc);
+                vx[i] = *reinterpret_cast<const uint4*>(vb + vo + 8 * lpc);
+            }
+        }
+    };
+    auto store = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int rw = (tid + i * kPagedThreads) / PR, lpc = (tid + i * kPagedThreads) % PR;
+            *reinterpret_cast<uint4*>(ks + (st & 1) * kTile + rw * LD + ((lpc ^ key_swz<LD>(rw)) << 3)) = kx[i];
+            *reinterpret_cast<uint4*>(vs + (st & 1) * kTile + rw * LD + ((lpc ^ value_swz<LD>(rw)) << 3)) = vx[i];
+        }
+    };
+
+    float m[QB], l[QB];
+    f32x16_t o[QB][DT];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        m[b] = -INFINITY;
+        l[b] = 0.f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[b][t][i] = 0.f;
+    }
+    unsigned long long have = 0;
+    if (steps > 0) {
+        if (wave < 2 && wave < steps) {
+            ask(wave);
+            locate(wave);
+        }
+        lds_publish_barrier();
+        have = __ballot(koff[0][lane] >= 0);
+        load(0);
+        store(0);
+        lds_publish_barrier();
+    }
+    for (int st = 0; st < steps; ++st) {
+        const int ub = r.u_lo + st * kChunkKeys;
+        unsigned long long have_next = 0;
+        const bool asks = st + 2 < steps && wave == (st & 3);
+        if (asks) ask(st + 2);
+        if (st + 1 < steps) {
+            have_next = __ballot(koff[(st + 1) & 1][lane] >= 0);
+            load(st + 1);
+        }
+        const T* const K = ks + (st & 1) * kTile;
+        const T* const V = vs + (st & 1) * kTile;
+        if (!idle && ub <= wl && ub + kChunkKeys - 1 >= some_lo) {
+            f32x16_t s[QB][2];
+#pragma unroll
+            for (int kb2 = 0; kb2 < 2; ++kb2) {
+                const int rw = 32 * kb2 + col;
+#pragma unroll
+                for (int b = 0; b < QB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[b][kb2][i] = 0.f;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const uint4 kf =
+                        *reinterpret_cast<const uint4*>(K + rw * LD + (((2 * c + h) ^ key_swz<LD>(rw)) << 3));
+#pragma unroll
+                    for (int b = 0; b < QB; ++b) s[b][kb2] = mma32<T>(kf, qf[b][c], s[b][kb2]);
+                }
+            }
+            if (have != ~0ull || ub + kChunkKeys - 1 > wf || ub < all_lo) {
+#pragma unroll
+                for (int b = 0; b < QB; ++b)
+#pragma unroll
+                    for (int kb2 = 0; kb2 < 2; ++kb2) {
+                        const uint32_t bits = static_cast<uint32_t>(have >> (32 * kb2)) >> (4 * h);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int k = 8 * (i / 4) + (i & 3), u = ub + 32 * kb2 + 4 * h + k;
+                            if (!((bits >> k) & 1) || u > hi[b] || u < lo[b]) s[b][kb2][i] = -INFINITY;
+                        }
+                    }
+            }
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                float top = fmaxp(s[b][0][0], s[b][1][0]);
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top = fmaxp(top, fmaxp(s[b][0][i], s[b][1][i]));
+                top = fmaxp(top, other_half(top)) * sp.sc2;
+                const float m2 = fmaxp(m[b], top), ref = m2 == -INFINITY ? 0.f : m2;
+                if (__ballot(m2 != m[b])) {
+                    const float keep = __builtin_amdgcn_exp2f(m[b] - ref);
+                    l[b] *= keep;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) o[b][t] *= keep;
+                }
+                m[b] = m2;
+                float sum = 0.f;
+#pragma unroll
+                for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[b][kb2][i] = __builtin_amdgcn_exp2f(fmaf(s[b][kb2][i], sp.sc2, -ref));
+                        sum += s[b][kb2][i];
+                    }
+                l[b] += sum;
+            }
+            // 16 keys at a time
+            const int vr = 4 * h + ((lane & 15) >> 2), vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                uint4 p[QB];
+#pragma unroll
+                for (int b = 0; b < QB; ++b) {
+                    const f32x16_t& x = s[b][kk >> 1];
+                    const int i0 = 8 * (kk & 1);
+                    p[b] = make_uint4(Mma<T>::pack(x[i0], x[i0 + 1]), Mma<T>::pack(x[i0 + 2], x[i0 + 3]),
+                                      Mma<T>::pack(x[i0 + 4], x[i0 + 5]), Mma<T>::pack(x[i0 + 6], x[i0 + 7]));
+                }
+                const int r0 = 16 * kk + vr, r1 = r0 + 8;
+                const T* const x0 = V + r0 * LD + (lane & 1) * 4;
+                const T* const x1 = V + r1 * LD + (lane & 1) * 4;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    const uint2 lo2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_i16x4_t*)(x0 + (((4 * t + vc) ^ value_swz<LD>(r0)) << 3))));
+                    const uint2 hi2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_i16x4_t*)(x1 + (((4 * t + vc) ^ value_swz<LD>(r1)) << 3))));
+                    const uint4 vf = make_uint4(lo2.x, lo2.y, hi2.x, hi2.y);
+#pragma unroll
+                    for (int b = 0; b < QB; ++b) o[b][t] = mma32<T>(vf, p[b], o[b][t]);
+                }
+            }
+        }
+        have = have_next;
+        if (st + 1 < steps) {
+            store(st + 1);
+            // the offsets of tile st + 2 replace those of tile st
+            if (asks) locate(st + 2);
+        }
+        lds_publish_barrier();
+    }
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const int rw = wrow + 32 * b + col;
+        if (rw >= r.rows) continue;
+        int qi, qh;
+        row_token(a, r.cls, r.h, r.row0 + rw, qi, qh);
+        const float lt = l[b] + other_half(l[b]);
+        float total = 0.f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) total += o[b][t][i];
+        if (item_nonfinite(total) && !item_nonfinite(m[b]) && !item_nonfinite(lt)) {
+            // as in k_paged_few: 0 times a value that is not finite
+            f32x4_t e[D / 8];
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) e[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            const T* const q = static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
+            for (int u = r.u_lo; u <= r.u_hi; ++u)
+                exact_key<T, D, D / 8, 8>(a, r, table, q, u, lo[b], hi[b], m[b], 4 * h, e);
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[b][n / 4][4 * (n & 3) + i] = e[n][i];
+        }
+        if (r.split) {
+            const long long at = static_cast<long long>(r.index) * a.M + rw;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float4*>(a.part + at * D + 8 * n + 4 * h) =
+                    make_float4(o[b][n / 4][4 * (n & 3)], o[b][n / 4][4 * (n & 3) + 1], o[b][n / 4][4 * (n & 3) + 2],
+                                o[b][n / 4][4 * (n & 3) + 3]);
+            if (h == 0) {
+                a.ml[2 * at] = m[b];
+                a.ml[2 * at + 1] = lt;
+            }
+            continue;
+        }
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        T* const out = static_cast<T*>(a.out) + r.b * a.lo.b + qi * a.lo.s2 + qh * a.lo.h;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<uint2*>(out + 8 * n + 4 * h) =
+                make_uint2(Mma<T>::pack(o[b][n / 4][4 * (n & 3)] * inv, o[b][n / 4][4 * (n & 3) + 1] * inv),
+                           Mma<T>::pack(o[b][n / 4][4 * (n & 3) + 2] * inv, o[b][n / 4][4 * (n & 3) + 3] * inv));
+        if (h == 0) a.lse[r.b * a.ll.b + qi * a.ll.s2 + qh * a.ll.h] = row_lse(m[b], lt);
+    }
+}
+
+// ---------------------------------------------------------------------------
 // joining parts
 // ---------------------------------------------------------------------------
 
-// A workgroup per row of a cut tile: 64 lanes on the head dims (in fours),
-// groups of lanes on different parts, joined through LDS in a fixed order.
+// Rows of tall tiles (few parts each): a group of lanes per row, the head dims
+// in fours, the parts in order.
+template <typename T>
+__global__ __launch_bounds__(kPagedThreads) void k_paged_join_rows(PagedArgs a) {
+    const int tile = blockIdx.x;
+    if (tile >= *a.count) return;
+    const PagedTile t = a.tiles[tile];
+    if (t.parts <= 1) return;
+    const int quads = a.Dv / 4, per = kPagedThreads / quads;
+    const int row = blockIdx.y * per + threadIdx.x / quads, d = 4 * (threadIdx.x % quads);
+    if (static_cast<int>(threadIdx.x) >= per * quads || row >= t.rows) return;
+    float m = -INFINITY;
+    for (int s = 0; s < t.parts; ++s)
+        m = fmaxp(m, a.ml[2 * ((static_cast<long long>(t.first) + static_cast<long long>(s) * t.step) * a.M + row)]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < t.parts; ++s) {
+        const long long at = (static_cast<long long>(t.first) + static_cast<long long>(s) * t.step) * a.M + row;
+        if (a.ml[2 * at] == -INFINITY && a.ml[2 * at + 1] == 0.f) continue;  // a part without keys
+        const float w = __builtin_amdgcn_exp2f(a.ml[2 * at] - ref);
+        l = fmaf(w, a.ml[2 * at + 1], l);
+        x += w * *reinterpret_cast<const f32x4_t*>(a.part + at * a.Dv + d);
+    }
+    int i, hq;
+    row_token(a, t.cls, t.h, t.row0 + row, i, hq);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* const out = static_cast<T*>(a.out) + t.b * a.lo.b + i * a.lo.s2 + hq * a.lo.h + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = from_f<T>(x[e] * inv);
+    if (d == 0) a.lse[t.b * a.ll.b + i * a.ll.s2 + hq * a.ll.h] = row_lse(m, l);
+}
+
+// Low tiles with many parts: a workgroup per row, groups of lanes on
+// different parts, joined through LDS in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(kPagedThreads) void k_paged_join(PagedArgs a) {
     __shared__ float o[kPagedThreads][5];
@@ -414,11 +743,11 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_join(PagedArgs a) {
     const int tid = threadIdx.x;
     float m = -INFINITY;
     for (int s = tid; s < t.parts; s += kPagedThreads)
-        m = fmaxf(m, a.ml[2 * ((static_cast<long long>(t.first) + static_cast<long long>(s) * t.step) * a.M + row)]);
-    for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+        m = fmaxp(m, a.ml[2 * ((static_cast<long long>(t.first) + static_cast<long long>(s) * t.step) * a.M + row)]);
+    for (int x = 32; x >= 1; x >>= 1) m = fmaxp(m, __shfl_xor(m, x));
     if ((tid & 63) == 0) o[tid >> 6][0] = m;
     lds_publish_barrier();
-    m = fmaxf(fmaxf(o[0][0], o[1][0]), fmaxf(o[2][0], o[3][0]));
+    m = fmaxp(fmaxp(o[0][0], o[1][0]), fmaxp(o[2][0], o[3][0]));
     const float ref = m == -INFINITY ? 0.f : m;
     __syncthreads();
     // quads of head dims on consecutive threads, the parts over the rest
@@ -471,7 +800,14 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_join(PagedArgs a) {
 // Workgroups aimed at when the tiles are few: two a compute unit.
 constexpr int kTarget = 512;
 
-enum PagedKind { kRows, kFew };
+// Rows of a class from which the tall tiles are taken.
+constexpr int kChunkFrom = 64;
+
+// 32-query blocks of a wave: two where their accumulators leave two waves a
+// SIMD (see k_paged_chunk).
+constexpr int chunk_blocks(int dim) { return dim <= 64 ? 2 : 1; }
+
+enum PagedKind { kRows, kFew, kChunk };
 
 struct PagedPlan {
     PagedKind kind;
@@ -494,8 +830,15 @@ bool on_mfma(const PagedCall& c) {
 
 PagedPlan plan(const PagedCall& c) {
     PagedPlan p{};
-    p.kind = on_mfma(c) ? kFew : kRows;
-    if (p.kind == kFew) {
+    const long long rep = c.heads_q / c.heads_kv;
+    const long long dil = c.dilation, classes = c.tokens < dil ? c.tokens : dil;
+    const long long members = (c.tokens + dil - 1) / dil;
+    p.kind = !on_mfma(c) ? kRows : members * rep < kChunkFrom ? kFew : kChunk;
+    if (p.kind == kChunk) {
+        p.M = 128 * chunk_blocks(c.dim_qk);
+        p.KT = kChunkKeys;
+        p.least = 8;
+    } else if (p.kind == kFew) {
         p.M = kFewRows;
         p.KT = 4 * kFewKeys;
         p.least = 2;
@@ -504,10 +847,6 @@ PagedPlan plan(const PagedCall& c) {
         p.KT = 64;
         p.least = 4;
     }
-    p.xcd_run = 0;
-    const long long rep = c.heads_q / c.heads_kv;
-    const long long dil = c.dilation, classes = c.tokens < dil ? c.tokens : dil;
-    const long long members = (c.tokens + dil - 1) / dil;
     const long long slots = classes * ((members * rep + p.M - 1) / p.M);
     p.slots = static_cast<int>(slots < 0x7fffffff ? slots : 0x7fffffff);
     p.tiles = slots * c.batch * c.heads_kv;
@@ -527,6 +866,11 @@ PagedPlan plan(const PagedCall& c) {
         p.bytes = padded(sizeof(int)) + padded(sizeof(PagedTile) * kTarget) +
                   padded(sizeof(float) * 2 * p.M * 2 * kTarget) + sizeof(float) * c.cache.dim_v * p.M * 2 * kTarget;
     }
+    if (p.kind == kChunk) {
+        // runs of tiles on one XCD, 4 or more on each; whole rounds of them
+        p.xcd_run = static_cast<int>(p.grid / 32 < 1 ? 1 : p.grid / 32 > 16 ? 16 : p.grid / 32);
+        p.grid = (p.grid + 8 * p.xcd_run - 1) / (8 * p.xcd_run) * (8 * p.xcd_run);
+    }
     return p;
 }
 
@@ -544,6 +888,17 @@ hipError_t launch_few(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <typename T, int D>
+hipError_t launch_chunk(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+    constexpr int lds = 2 * 2 * kChunkKeys * row_elems<D>() * sizeof(T);
+    const auto kernel = k_paged_chunk<T, D, chunk_blocks(D)>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+    NA_LAUNCH("na_paged_chunk", kernel, dim3(p.grid), dim3(kPagedThreads), lds, s, a);
+    return hipGetLastError();
+}
+
 template <typename T>
 hipError_t launch_kind(const PagedArgs& a, const PagedPlan& p, bool vec, hipStream_t s) {
     hipError_t e = hipSuccess;
@@ -555,9 +910,19 @@ hipError_t launch_kind(const PagedArgs& a, const PagedPlan& p, bool vec, hipStre
             NA_LAUNCH("na_paged_rows", (k_paged_rows<T, 1>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
         e = hipGetLastError();
     } else if constexpr (!std::is_same<T, float>::value) {
-        e = launch_few<T>(a, p, s);
+        if (p.kind == kFew) e = launch_few<T>(a, p, s);
+        else if (a.Dqk == 32) e = launch_chunk<T, 32>(a, p, s);
+        else if (a.Dqk == 64) e = launch_chunk<T, 64>(a, p, s);
+        else if (a.Dqk == 96) e = launch_chunk<T, 96>(a, p, s);
+        else e = launch_chunk<T, 128>(a, p, s);
     }
     if (e != hipSuccess || !p.split) return e;
+    if (p.kind == kChunk) {
+        const int per = kPagedThreads / (a.Dv / 4);
+        NA_LAUNCH("na_paged_join", (k_paged_join_rows<T>),
+                  dim3(p.tiles < kTarget ? p.tiles : kTarget, (p.M + per - 1) / per), dim3(kPagedThreads), 0, s, a);
+        return hipGetLastError();
+    }
     NA_LAUNCH("na_paged_join", (k_paged_join<T>), dim3(p.tiles < kTarget ? p.tiles : kTarget, p.M),
               dim3(kPagedThreads), 0, s, a);
     return hipGetLastError();
