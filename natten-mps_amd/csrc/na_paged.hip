@@ -892,9 +892,6 @@ template <typename T, int D>
 hipError_t launch_chunk(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
     constexpr int lds = 2 * 2 * kChunkKeys * row_elems<D>() * sizeof(T);
     const auto kernel = k_paged_chunk<T, D, chunk_blocks(D)>;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
     NA_LAUNCH("na_paged_chunk", kernel, dim3(p.grid), dim3(kPagedThreads), lds, s, a);
     return hipGetLastError();
 }

@@ -32,6 +32,9 @@
 // innermost stride, lse / dlse that are not contiguous fp32, parameters that
 // are not sequences of ints).
 //
+// Rotary positions and the paged cache (na_torch_paged.h) check an ordinary
+// call in C++ and need no registered signature.
+//
 // Reference: the backend hooks this serves are those the autograd factory
 // calls (autograd/_factory.py:37-38,66-67 of /root/reference/src/natten_mps)
 // the split ops' forward and backward hooks (_core/ops.py:98-152), and the
@@ -44,6 +47,8 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <optional>
 #include <string>
@@ -819,6 +824,8 @@ bool split_register(int64_t rank, const std::vector<at::Tensor>& ts, pybind11::h
 
 }  // namespace
 
+#include "na_torch_paged.h"
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "Host binding of the fused and split entry points for the 'hip' backend";
     m.attr("abi_version") = natten_hip_abi_version();
@@ -867,6 +874,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("av_bwd", &av_bwd, "cached split AV backward: (dattn, dv), or None");
     m.def("split_register", &split_register,
           "register the SplitCall of a split-op signature (its input tensors in the op's argument order)");
+    m.def("rotary", &rotary, "q (and k) turned by their positions, with gradients, or None");
+    m.def("paged_append", &paged_append, "new tokens into a paged cache: (turned q,) or (), or None");
+    m.def("paged_forward", &paged_forward, "attention over a paged cache: (out, lse), or None");
     m.def("clear", &clear_all, "drop every registered signature");
     // the cached objects hold Python references: release them before the
     // interpreter's own teardown

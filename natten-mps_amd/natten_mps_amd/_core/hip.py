@@ -933,6 +933,35 @@ def _axis_lay(t: torch.Tensor) -> "_lib.Layout":
     return _lib.layout(t, t.ndim - 3, 1)
 
 
+def rotary_call(q, k, plan, positions):
+    """Turned tensors of an ordinary call, with gradients, through the host
+    binding; None where positions.py has to look at the arguments."""
+    b = _lib.binding()
+    if b is None:
+        return None
+    return b.rotary(q, k, positions, plan.table(q.device), plan.dim, plan.axes, plan.interleaved, plan.magnitude)
+
+
+def paged_append_call(key, value, key_pages, value_pages, table, seq_lens, new_lens, query, plan):
+    """(turned query,) or () of an ordinary call, None otherwise."""
+    b = _lib.binding()
+    if b is None:
+        return None
+    if plan is None:
+        return b.paged_append(key, value, key_pages, value_pages, table, seq_lens, new_lens, query, None, 0, 1, False,
+                              1.0)
+    return b.paged_append(key, value, key_pages, value_pages, table, seq_lens, new_lens, query,
+                          plan.table(key.device), plan.dim, plan.axes, plan.interleaved, plan.magnitude)
+
+
+def paged_forward_call(query, key_pages, value_pages, table, seq_lens, new_lens, kernel_size, dilation, scale):
+    """(out, lse) of an ordinary call, None otherwise."""
+    b = _lib.binding()
+    if b is None:
+        return None
+    return b.paged_forward(query, key_pages, value_pages, table, seq_lens, new_lens, kernel_size, dilation, scale)
+
+
 def rotary(q, k, plan, positions, inverse):
     """``(q', k')``: q and k (None: absent) turned by their positions."""
     _on_device(q, k, positions)

@@ -37,6 +37,13 @@ def _hook(name: str):
     return fn
 
 
+def _call(name: str, x):
+    """The backend's check and run of an ordinary call, where it has one."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        return None
+    return getattr(ops.active_module(), name, None)
+
+
 def _no_grad(what: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradients: call it under torch.no_grad() or detach its tensors.")
@@ -75,6 +82,11 @@ def na1d_paged_append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.T
     values).  Returns None without a query.  Other slots of the pages, and
     those of padding tokens, stay as they are; ``key`` and ``value`` must not
     overlap the pages."""
+    fn = _call("paged_append_call", key)
+    if fn is not None and (plan is None or type(plan) is RotaryPlan):
+        done = fn(key, value, key_pages, value_pages, block_table, seq_lens, new_lens, query, plan)
+        if done is not None:
+            return done[0] if done else None
     what = "na1d_paged_append"
     if key.ndim != 4 or value.ndim != 4 or key.shape[:3] != value.shape[:3]:
         raise ValueError(f"{what} expects key and value with shape [B, L, heads_kv, dim], matching but for their "
@@ -113,6 +125,11 @@ def na1d_paged(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.
     heads]`` in float32 when ``return_lse`` (with which
     :func:`~natten_mps_amd.merge_attentions` adds other keys).  Padding
     tokens, and queries without a key, have zeros and an lse of -inf."""
+    fn = _call("paged_forward_call", query)
+    if fn is not None:
+        done = fn(query, key_pages, value_pages, block_table, seq_lens, new_lens, kernel_size, dilation, scale)
+        if done is not None:
+            return done if return_lse else done[0]
     what = "na1d_paged"
     if query.ndim != 4:
         raise ValueError(f"{what} expects query with shape [B, L, heads, dim], got {tuple(query.shape)}.")

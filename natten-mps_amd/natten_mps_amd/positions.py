@@ -230,6 +230,14 @@ def _hook():
     return fn
 
 
+def _call(x, key, plan, positions):
+    """An ordinary call, checked and run by the backend; None otherwise."""
+    if type(plan) is not RotaryPlan or not isinstance(x, torch.Tensor) or not x.is_cuda:
+        return None
+    fn = getattr(ops.active_module(), "rotary_call", None)
+    return None if fn is None else fn(x, key, plan, positions)
+
+
 def _turn(plan, positions, *tensors):
     hook = _hook()
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
@@ -244,6 +252,9 @@ def rotary(x: torch.Tensor, plan: RotaryPlan, positions: Optional[torch.Tensor] 
     ``positions``: None for the tokens' own indices (one plan axis per
     spatial axis), or int32 / int64 ``[*spatial]`` or ``[B, *spatial]``, with
     a trailing dim of coordinates when the plan has several axes."""
+    done = _call(x, None, plan, positions)
+    if done is not None:
+        return done[0]
     _check_tensor(x, "a tensor")
     check_plan(plan, x.shape[-1])
     _check_positions(positions, plan, x.shape)
@@ -254,6 +265,9 @@ def rotary_qk(query: torch.Tensor, key: torch.Tensor, plan: RotaryPlan,
               positions: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`rotary` of queries and keys in one launch; they may differ in
     their number of heads only."""
+    done = _call(query, key, plan, positions)
+    if done is not None:
+        return done
     _check_tensor(query, "query")
     _check_tensor(key, "key")
     if query.shape[:-2] != key.shape[:-2] or query.shape[-1] != key.shape[-1]:

@@ -554,3 +554,31 @@ def test_captured_steps_follow_the_cache():
         for got in outs:
             for a, b in zip(got, want):
                 assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_without_the_host_binding(dtype, monkeypatch):
+    """The ctypes calls give what the C++ host binding gives."""
+    from natten_mps_amd._core import _lib
+
+    plan = na.RotaryPlan(32, scaling="linear", factor=4)
+    p = Problem([(3, 700), (40, 90)], 4, 2, 64, 16, dtype)
+    k, v = _randn(1, 2, 40, 2, 64, dtype=dtype), _randn(2, 2, 40, 2, 64, dtype=dtype)
+    pos = torch.arange(80, device=DEV).view(2, 40)
+    leaf, g = _randn(3, 2, 40, 2, 64, dtype=dtype).requires_grad_(), _randn(4, 2, 40, 2, 64, dtype=dtype)
+
+    def calls():
+        kp, vp = p.kp.clone(), p.vp.clone()
+        q = na.na1d_paged_append(k, v, kp, vp, p.table, p.lens, p.news, query=p.q, plan=plan)
+        plain = na.na1d_paged_append(k, v, kp, vp, p.table, p.lens, p.news, query=p.q)
+        att = na.na1d_paged(q, kp, vp, p.table, p.lens, 300, 2, new_lens=p.news, return_lse=True)
+        every = na.na1d_paged(q, kp, vp, p.table, p.lens, new_lens=p.news)
+        out = na.rotary(leaf, plan, pos)
+        both = na.rotary_qk(leaf, g, plan)
+        return (q, plain, kp, vp, *att, every, out, *both, *torch.autograd.grad(out, leaf, g),
+                *torch.autograd.grad(both[0], leaf, g))
+
+    with_binding = calls()
+    monkeypatch.setattr(_lib, "binding", lambda: None)
+    for a, b in zip(with_binding, calls()):
+        assert torch.equal(a, b)
