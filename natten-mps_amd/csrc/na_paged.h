@@ -33,19 +33,19 @@ struct PagedArgs {
     long long kp, ks, kh, vp, vs, vh;
     const int *table, *lens, *news;
     long long table_stride;
-    int width, pages, page_size;
+    int cap, pages, page_size;  // cap: positions of the table, an int at most
     FastDiv fpage;
     int B, L, Hq, Hkv, rep, Dqk, Dv;
-    FastDiv frep;
+    FastDiv frep, flen, fdv;
     int K, dil;  // K 0: no window
     FastDiv fdil;
     float scale;
-    int M, KT;           // rows of a tile, keys of a block
-    int tile_slots;      // tiles of a (sequence, kv head) at most
-    int direct;          // every tile whole: slot = tile, nothing to work out
-    int target;          // workgroups aimed at when tiles are few
-    int least;           // key blocks of a chunk at least
-    int xcd_run;         // consecutive shares of one XCD (0: as dealt)
+    int M, log_m, log_kt;  // rows of a tile, keys of a block
+    int tile_slots;        // tiles of a (sequence, kv head) at most
+    int direct;            // every tile whole: slot = tile, nothing to work out
+    int log_target;        // workgroups aimed at when tiles are few
+    int least;             // key blocks of a chunk at least
+    int xcd_run;           // consecutive shares of one XCD (0: as dealt)
     FastDiv fslots, fkv, frun;
     // split tiles: header (count of tiles), a record per tile, m and l, O
     int* count;
@@ -60,28 +60,29 @@ struct PagedTile {
     int b, h, cls, row0, rows;
 };
 
+// Divisions are by invariants (FastDiv) or powers of two: an emulated 64-bit
+// one costs half a microsecond of a call's latency.
 struct SeqGeo {
-    int n, len, classes, tiles, blocks;  // tiles: of all its classes, one kv head
+    int n, len, classes, per_class, tiles, blocks;  // tiles: of all its classes, one kv head
 };
 
-// ceil(a / b) of a >= 0 for any b >= 1 (a dilation may be as large as an int).
-__device__ __forceinline__ int ceil_div(int a, int b) { return a > 0 ? (a - 1) / b + 1 : 0; }
+// ceil(n / d) of 0 <= n
+__device__ __forceinline__ int ceil_fdiv(int n, const FastDiv& d) { return n > 0 ? fdiv(n - 1, d) + 1 : 0; }
 
-__device__ __forceinline__ SeqGeo seq_geo(const PagedArgs& a, int b) {
+__device__ __forceinline__ SeqGeo seq_geo(const PagedArgs& a, int n, int len) {
     SeqGeo g;
-    g.n = a.news ? imin(imax(a.news[b], 0), a.L) : a.L;
-    g.len = imax(a.lens[b], 0);
+    g.n = imin(imax(n, 0), a.L);
+    g.len = imax(len, 0);
     g.classes = imin(g.n, a.dil);
-    const int members = ceil_div(g.n, a.dil);
-    const int per_class = ceil_div(members * a.rep, a.M);
-    g.tiles = g.classes * per_class;
-    const long long cap = static_cast<long long>(a.width) * a.page_size;
-    long long keys = (g.len < cap ? g.len : cap) / a.dil + 1;
+    const int members = ceil_fdiv(g.n, a.fdil);
+    g.per_class = (members * a.rep + a.M - 1) >> a.log_m;
+    g.tiles = g.classes * g.per_class;
+    int keys = fdiv(imin(g.len, a.cap), a.fdil) + 1;
     if (a.K) {
-        const long long span = static_cast<long long>(a.K) + imin(members, a.M / a.rep + 2) - 1;
-        if (span < keys) keys = span;
+        const uint32_t span = static_cast<uint32_t>(a.K) + imin(members, fdiv(a.M, a.frep) + 2) - 1;
+        if (span < static_cast<uint32_t>(keys)) keys = static_cast<int>(span);
     }
-    g.blocks = static_cast<int>((keys + a.KT - 1) / a.KT);
+    g.blocks = ((keys - 1) >> a.log_kt) + 1;
     return g;
 }
 
@@ -95,22 +96,33 @@ struct Share {
     bool split;
 };
 
-// Sum over the workgroup; `red` has 4 entries per call site's use.
-__device__ __forceinline__ long long block_sum(long long v, long long* red) {
-    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    lds_publish_barrier();
-    return red[0] + red[1] + red[2] + red[3];
+// Inclusive running sums over the wave's lanes (DPP shifts inside 16-lane
+// rows, then the rows' last lanes to the rows after them).
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp_or_zero(T v) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, true));
 }
 
-struct ShareScratch {
-    long long red[4];
-    int found[8];
-};
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp_or_zero<0x111, 0xf>(v);
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);
+    v += dpp_or_zero<0x143, 0xc>(v);
+    return v;
+}
 
-__device__ __forceinline__ bool find_share(const PagedArgs& a, ShareScratch& sh, Share& r) {
-    const int tid = threadIdx.x;
+template <typename T>
+__device__ __forceinline__ T lane_value(T v, int lane) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+// Every wave works the cut out for itself, lanes on sequences, 64 at a time:
+// no barriers, and what comes out is uniform.
+__device__ __forceinline__ bool find_share(const PagedArgs& a, Share& r) {
+    const int lane = threadIdx.x & 63, target = 1 << a.log_target;
     int want = blockIdx.x;
     if (a.xcd_run) {
         // workgroups are dealt to the 8 XCDs in turn: give each XCD runs of
@@ -118,120 +130,123 @@ __device__ __forceinline__ bool find_share(const PagedArgs& a, ShareScratch& sh,
         const int slot = want >> 3, run = fdiv(slot, a.frun);
         want = (run * 8 + (want & 7)) * a.xcd_run + (slot - run * a.xcd_run);
     }
-    int b, rem, parts = 1, chunk = 0, tiles, first = 0;
-    SeqGeo g;
+    int b, rem, parts = 1, chunk = 0, tile_first = 0, n, len;
+    r.h = 0;
+    r.split = false;
+    r.index = 0;
     if (a.direct) {
         const int bh = fdiv(want, a.fslots);
         rem = want - bh * a.tile_slots;
         b = fdiv(bh, a.fkv);
         if (b >= a.B) return false;
         r.h = bh - b * a.Hkv;
-        g = seq_geo(a, b);
-        if (rem >= g.tiles) return false;
-        tiles = g.tiles;
-        r.split = false;
-        r.index = 0;
+        n = a.news ? a.news[b] : a.L;
+        len = a.lens[b];
     } else {
-        // tiles and key blocks of the whole batch
-        long long work = 0, all = 0;
-        for (int i = tid; i < a.B; i += kPagedThreads) {
-            const SeqGeo s = seq_geo(a, i);
-            all += static_cast<long long>(s.tiles) * a.Hkv;
-            work += static_cast<long long>(s.tiles) * a.Hkv * s.blocks;
-        }
-        all = block_sum(all, sh.red);
-        work = block_sum(work, sh.red);
-        chunk = 0x7fffffff;
-        if (all < a.target) {
-            const long long c = (work + a.target - 1) / a.target;
-            chunk = static_cast<int>(c > a.least ? c : a.least);
-        }
-        if (blockIdx.x == 0 && tid == 0) *a.count = all < a.target ? static_cast<int>(all) : 0;
-        // the sequence whose shares hold `want`: running sums, 256 at a time
-        if (tid == 0) sh.found[0] = -1;
-        long long base = 0, tile_base = 0;
-        for (int i0 = 0; i0 < a.B; i0 += kPagedThreads) {
-            const int i = i0 + tid;
-            int mine = 0, mine_tiles = 0, ns = 1;
+        // tiles and key blocks of the whole batch; the sum of blocks in fp32,
+        // so that the chunk from it is one more than rounding can lose
+        int all = 0;
+        float work = 0.f;
+        int n0 = 0, len0 = 0;  // of the first 64 sequences
+        for (int i0 = 0; i0 < a.B; i0 += 64) {
+            const int i = i0 + lane;
+            int ni = 0, li = 0;
             if (i < a.B) {
-                const SeqGeo s = seq_geo(a, i);
-                ns = chunk == 0x7fffffff ? 1 : (s.blocks + chunk - 1) / chunk;
-                mine_tiles = s.tiles * a.Hkv;
-                mine = mine_tiles * ns;
+                ni = a.news ? a.news[i] : a.L;
+                li = a.lens[i];
             }
-            int run = mine, run_tiles = mine_tiles;
-            for (int m = 1; m < 64; m <<= 1) {
-                const int x = __shfl_up(run, m), y = __shfl_up(run_tiles, m);
-                if ((tid & 63) >= m) {
-                    run += x;
-                    run_tiles += y;
-                }
+            if (i0 == 0) {
+                n0 = ni;
+                len0 = li;
             }
-            __syncthreads();
-            if ((tid & 63) == 63) sh.red[tid >> 6] = (static_cast<long long>(run_tiles) << 32) | static_cast<uint32_t>(run);
-            lds_publish_barrier();
-            long long lo = base, tlo = tile_base;
-            for (int w = 0; w < 4; ++w) {
-                const int items = static_cast<int>(sh.red[w] & 0xffffffff), tl = static_cast<int>(sh.red[w] >> 32);
-                if (w < (tid >> 6)) {
-                    lo += items;
-                    tlo += tl;
-                }
-                base += items;
-                tile_base += tl;
-            }
-            lo += run - mine;
-            if (want >= lo && want < lo + mine) {
-                sh.found[0] = i;
-                sh.found[1] = want - static_cast<int>(lo);
-                sh.found[2] = ns;
-                sh.found[3] = static_cast<int>(lo);
-                sh.found[4] = static_cast<int>(tlo + run_tiles - mine_tiles);
-            }
-            if (base > want) break;
+            const SeqGeo s = seq_geo(a, ni, li);
+            const int tiles = s.tiles * a.Hkv;
+            all += lane_value(wave_scan(tiles), 63);
+            work += lane_value(wave_scan(static_cast<float>(tiles) * static_cast<float>(s.blocks)), 63);
         }
-        lds_publish_barrier();
-        b = sh.found[0];
-        if (b < 0) return false;
-        rem = sh.found[1];
-        parts = sh.found[2];
-        first = sh.found[3];
-        g = seq_geo(a, b);
-        tiles = g.tiles;
-        // order: kv head, part, tile
-        const int per_head = parts * tiles;
-        r.h = rem / per_head;
-        rem -= r.h * per_head;
+        const bool cut = all < target;
+        chunk = imax(static_cast<int>(__builtin_ldexpf(work, -a.log_target)) + 1, a.least);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = cut ? all : 0;
+        // the sequence whose shares hold `want`.  Where keys are cut there are
+        // fewer than 2^9 tiles and 2^10 shares, summed together.
+        int base = 0, owner = -1, lo = 0, ns = 1;
+        int i0 = 0;
+        for (; i0 < a.B; i0 += 64) {
+            const int i = i0 + lane;
+            int ni = n0, li = len0;
+            if (i0) {
+                ni = li = 0;
+                if (i < a.B) {
+                    ni = a.news ? a.news[i] : a.L;
+                    li = a.lens[i];
+                }
+                n0 = ni;
+                len0 = li;
+            }
+            const SeqGeo s = seq_geo(a, ni, li);
+            ns = cut ? static_cast<int>(static_cast<uint32_t>(s.blocks + chunk - 1) / static_cast<uint32_t>(chunk)) : 1;
+            const int tiles = s.tiles * a.Hkv;
+            const int sum = wave_scan(cut ? (tiles << 16) + tiles * ns : tiles);
+            lo = base + sum - (cut ? (tiles << 16) + tiles * ns : tiles);
+            const int mine = cut ? lo & 0xffff : lo;
+            const unsigned long long hit = __ballot(i < a.B && want >= mine && want < mine + tiles * ns);
+            if (hit) {
+                owner = __ffsll(hit) - 1;
+                // parts of one tile as even as whole blocks allow
+                chunk = ns == 1 ? 0 : static_cast<int>(static_cast<uint32_t>(s.blocks + ns - 1) / static_cast<uint32_t>(ns));
+                break;
+            }
+            base += lane_value(sum, 63);
+        }
+        if (owner < 0) return false;
+        b = i0 + owner;
+        n = lane_value(n0, owner);
+        len = lane_value(len0, owner);
+        parts = lane_value(ns, owner);
+        chunk = lane_value(chunk, owner);
+        const int at = lane_value(lo, owner);
+        rem = want - (cut ? at & 0xffff : at);
+        tile_first = cut ? at >> 16 : at;
         r.split = parts > 1;
         r.index = want;
     }
-    const int part = rem / tiles, slot = rem - part * tiles;
-    const int per_class = tiles / g.classes;
+    const SeqGeo g = seq_geo(a, __builtin_amdgcn_readfirstlane(n), __builtin_amdgcn_readfirstlane(len));
+    if (a.direct) {
+        if (rem >= g.tiles) return false;
+    } else {
+        // order: kv head, part, tile
+        const int per_head = parts * g.tiles;
+        r.h = static_cast<int>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(per_head));
+        rem -= r.h * per_head;
+    }
+    int part = 0, slot = rem;
+    if (parts > 1) {
+        part = static_cast<int>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(g.tiles));
+        slot = rem - part * g.tiles;
+    }
     r.b = b;
     r.n = g.n;
-    r.cls = slot / per_class;
+    r.cls = g.classes == 1 ? 0 : static_cast<int>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(g.per_class));
     // the last tiles have the most keys: first
-    const int t = per_class - 1 - (slot - r.cls * per_class);
-    const int members = ceil_div(g.n - r.cls, a.dil);
-    r.row0 = t * a.M;
+    const int t = g.per_class - 1 - (slot - r.cls * g.per_class);
+    const int members = ceil_fdiv(g.n - r.cls, a.fdil);
+    r.row0 = t << a.log_m;
     r.rows = imin(a.M, members * a.rep - r.row0);
     const int x = g.len - g.n + r.cls;  // position of member 0
-    r.w0 = x >= 0 ? fdiv(x, a.fdil) : -((-x - 1) / a.dil + 1);
+    r.w0 = x >= 0 ? fdiv(x, a.fdil) : -(fdiv(-x - 1, a.fdil) + 1);
     r.c = x - r.w0 * a.dil;
     r.u_lo = 0;
     r.u_hi = -1;
     if (r.rows > 0) {
         const int wf = r.w0 + fdiv(r.row0, a.frep), wl = r.w0 + fdiv(r.row0 + r.rows - 1, a.frep);
         r.u_lo = a.K ? imax(0, wf - a.K + 1) : 0;
-        const long long cap = static_cast<long long>(a.width) * a.page_size - 1 - r.c;
-        const long long last = cap < 0 ? -1 : cap / a.dil;
-        r.u_hi = wl < last ? wl : static_cast<int>(last);
+        r.u_hi = imin(wl, r.c < a.cap ? fdiv(a.cap - 1 - r.c, a.fdil) : -1);
     }
     if (r.split) {
-        if (part == 0 && tid == 0) {
-            PagedTile& p = a.tiles[sh.found[4] + r.h * tiles + slot];
+        if (part == 0 && threadIdx.x == 0) {
+            PagedTile& p = a.tiles[tile_first + r.h * g.tiles + slot];
             p.first = want;
-            p.step = tiles;
+            p.step = g.tiles;
             p.parts = parts;
             p.b = b;
             p.h = r.h;
@@ -239,15 +254,16 @@ __device__ __forceinline__ bool find_share(const PagedArgs& a, ShareScratch& sh,
             p.row0 = r.row0;
             p.rows = r.rows;
         }
-        const long long from = r.u_lo + static_cast<long long>(part) * chunk * a.KT;
-        const long long to = from + static_cast<long long>(chunk) * a.KT - 1;
-        if (from > r.u_hi) r.u_hi = r.u_lo - 1;
-        else {
+        const int keys = chunk << a.log_kt;
+        const long long from = r.u_lo + static_cast<long long>(part) * keys;
+        if (from > r.u_hi) {
+            r.u_hi = r.u_lo - 1;
+        } else {
             r.u_lo = static_cast<int>(from);
-            if (to < r.u_hi) r.u_hi = static_cast<int>(to);
+            if (from + keys - 1 < r.u_hi) r.u_hi = static_cast<int>(from + keys - 1);
         }
-    } else if (!a.direct && tid == 0 && sh.found[4] + r.h * tiles + slot < a.target) {
-        a.tiles[sh.found[4] + r.h * tiles + slot].parts = 1;
+    } else if (!a.direct && threadIdx.x == 0 && tile_first + r.h * g.tiles + slot < target) {
+        a.tiles[tile_first + r.h * g.tiles + slot].parts = 1;
     }
     return true;
 }

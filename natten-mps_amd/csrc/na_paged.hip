@@ -30,11 +30,11 @@ __device__ __forceinline__ void clear_padding(const PagedArgs& a) {
     if (!a.news) return;
     const int tokens = a.B * a.L;
     for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
-        const int b = t / a.L, i = t - b * a.L;
+        const int b = fdiv(t, a.flen), i = t - b * a.L;
         if (i < a.news[b]) continue;
         T* const o = static_cast<T*>(a.out) + b * a.lo.b + i * a.lo.s2;
         for (int e = threadIdx.x; e < a.Hq * a.Dv; e += kPagedThreads) {
-            const int h = e / a.Dv;
+            const int h = fdiv(e, a.fdv);
             o[h * a.lo.h + (e - h * a.Dv)] = from_f<T>(0.f);
         }
         for (int h = threadIdx.x; h < a.Hq; h += kPagedThreads)
@@ -60,11 +60,10 @@ __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -
 // the products.  `VEC` elements of a key are read at once.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kPagedThreads) void k_paged_rows(PagedArgs a) {
-    __shared__ ShareScratch sh;
     __shared__ float qs[4][256];
     clear_padding<T>(a);
     Share r;
-    if (!find_share(a, sh, r)) return;
+    if (!find_share(a, r)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (wave >= r.rows) return;
     int i, hq;
@@ -179,27 +178,37 @@ __device__ __forceinline__ uint4 scaled(uint4 x, const ScaleParts& s) {
                       (x.w & s.keep) ^ s.flip);
 }
 
-// One key's part of a row's products, in plain arithmetic: acc[e] += p v[dv]
-// for `N` runs of four head dims from dv0 in steps of `step`.  Keys and pages
-// that the row does not attend to are not touched.
-template <typename T, int D, int N, int STEP>
-__device__ __forceinline__ void exact_key(const PagedArgs& a, const Share& r, const int* table, const T* q, int u,
-                                          int lo, int hi, float m, int dv0, f32x4_t (&acc)[N]) {
-    int page, slot;
-    if (u < lo || u > hi || !key_at(a, table, r.c, u, r.u_hi, page, slot)) return;
-    const T* const k = static_cast<const T*>(a.k) + (page * a.kp + slot * a.ks + r.h * a.kh);
-    const T* const v = static_cast<const T*>(a.v) + (page * a.vp + slot * a.vs + r.h * a.vh) + dv0;
-    float dot = 0.f;
-#pragma unroll 4
-    for (int d = 0; d < D; ++d) dot = fmaf(to_f(q[d]), to_f(k[d]), dot);
-    const float p = __builtin_amdgcn_exp2f(dot * (a.scale * kLog2e) - m);
+// Four head dims of a row, key by key in plain arithmetic: where a value that
+// is not finite met a probability of 0 in a product, rows of the tile that do
+// not attend to that key got NaN.  Keys that the row does not attend to are
+// not touched here.  Not normalised; m the row's maximum (base 2).
+template <typename T, int D>
+__device__ __forceinline__ f32x4_t exact_four(const PagedArgs& a, const Share& r, int row, float m, int d) {
+    int qi, qh;
+    row_token(a, r.cls, r.h, r.row0 + row, qi, qh);
+    const T* const q = static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
+    const int w = r.w0 + fdiv(r.row0 + row, a.frep);
+    const int* const table = a.table + r.b * a.table_stride;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int u = imax(r.u_lo, a.K ? w - a.K + 1 : 0); u <= imin(r.u_hi, w); ++u) {
+        int page, slot;
+        if (!key_at(a, table, r.c, u, r.u_hi, page, slot)) continue;
+        const T* const k = static_cast<const T*>(a.k) + (page * a.kp + slot * a.ks + r.h * a.kh);
+        const T* const v = static_cast<const T*>(a.v) + (page * a.vp + slot * a.vs + r.h * a.vh) + d;
+        float dot = 0.f;
+#pragma unroll 1
+        for (int x = 0; x < D; ++x) dot = fmaf(to_f(q[x]), to_f(k[x]), dot);
+        const float p = __builtin_amdgcn_exp2f(dot * (a.scale * kLog2e) - m);
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(p, to_f(v[n * STEP + i]), acc[n][i]);
+        for (int i = 0; i < 4; ++i) acc[i] = fmaf(p, to_f(v[i]), acc[i]);
+    }
+    return acc;
 }
 
-// 16 rows, the four waves on different keys, 32 at a time each.
+__device__ __forceinline__ bool four_nonfinite(f32x4_t x) { return item_nonfinite((x[0] + x[1]) + (x[2] + x[3])); }
+
+// 16 NB rows, the four waves on different keys, 32 at a time each.
 //
 // Scores as S^T = K Q^T (v_mfma 16x16x32): a lane then holds one query (its
 // column) and keys 4g..4g+3 of each 16-key block (g its 16-lane row), so the
@@ -214,35 +223,42 @@ __device__ __forceinline__ void exact_key(const PagedArgs& a, const Share& r, co
 // page numbers one step before that.
 constexpr int kFewRows = 16, kFewKeys = 32;
 
-template <typename T, int D>
+template <typename T, int D, int NB>
 __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
     constexpr int C = D / 32, LD = row_elems<D>(), DB = D / 16;
-    __shared__ ShareScratch sh;
-    __shared__ __attribute__((aligned(16))) T vs[4][kFewKeys * LD];
-    __shared__ float ml[4][kFewRows][2];
+    constexpr int kRowsOf = kFewRows * NB;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ float ml[4][kRowsOf][2];
     clear_padding<T>(a);
     Share r;
-    if (!find_share(a, sh, r)) return;
+    if (!find_share(a, r)) return;
     if (r.rows <= 0) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int col = lane & 15, g = lane >> 4;
-    const int row = r.row0 + imin(col, r.rows - 1);
-    int qi, qh;
-    row_token(a, r.cls, r.h, row, qi, qh);
-    const T* const q = static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
     const ScaleParts sp = scale_parts(a.scale);
-    uint4 qf[C];
+    // queries, their windows, and what all rows of the tile see
+    uint4 qf[NB][C];
+    int hi[NB], lo[NB];
+    auto query = [&](int n) {
+        int qi, qh;
+        row_token(a, r.cls, r.h, r.row0 + imin(16 * n + col, r.rows - 1), qi, qh);
+        return static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
+    };
 #pragma unroll
-    for (int c = 0; c < C; ++c) qf[c] = scaled(*reinterpret_cast<const uint4*>(q + 32 * c + 8 * g), sp);
-    // the row's window, and what all rows of the tile see
-    const int hi = r.w0 + fdiv(row, a.frep), lo = a.K ? hi - a.K + 1 : 0;
+    for (int n = 0; n < NB; ++n) {
+        const T* const q = query(n);
+#pragma unroll
+        for (int c = 0; c < C; ++c) qf[n][c] = scaled(*reinterpret_cast<const uint4*>(q + 32 * c + 8 * g), sp);
+        hi[n] = r.w0 + fdiv(r.row0 + imin(16 * n + col, r.rows - 1), a.frep);
+        lo[n] = a.K ? hi[n] - a.K + 1 : 0;
+    }
     const int all_hi = imin(r.w0 + fdiv(r.row0, a.frep), r.u_hi);
     const int all_lo = a.K ? r.w0 + fdiv(r.row0 + r.rows - 1, a.frep) - a.K + 1 : 0;
     const int steps = (r.u_hi - r.u_lo + kFewKeys) / kFewKeys;  // 0 when empty: u_hi = u_lo - 1 at least
     const int* const table = a.table + r.b * a.table_stride;
     const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh + 8 * g;
     const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh + 8 * g;
-    T* const X = vs[wave];
+    T* const X = reinterpret_cast<T*>(lds) + wave * (kFewKeys * LD);
 
     int page[2], slot[2];
     auto lookup = [&](int st) {
@@ -272,10 +288,15 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
         }
     };
 
-    float m = -INFINITY, l = 0.f;
-    f32x4_t o[DB];
+    float m[NB], l[NB];
+    f32x4_t o[NB][DB];
 #pragma unroll
-    for (int db = 0; db < DB; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NB; ++n) {
+        m[n] = -INFINITY;
+        l[n] = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[n][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
     if (wave < steps) {
         lookup(wave);
         load(wave);
@@ -283,13 +304,15 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
     }
     for (int st = wave; st < steps; st += 4) {
         const int ub = r.u_lo + st * kFewKeys;
-        f32x4_t s[2];
+        f32x4_t s[NB][2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            s[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int c = 0; c < C; ++c) s[b] = Mma<T>::run(kf[b][c], qf[c], s[b]);
-        }
+            for (int b = 0; b < 2; ++b) {
+                s[n][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < C; ++c) s[n][b] = Mma<T>::run(kf[b][c], qf[n][c], s[n][b]);
+            }
         const bool there[2] = {ok[0], ok[1]};
         const unsigned long long have0 = __ballot(there[0]), have1 = __ballot(there[1]);
         const bool whole = (have0 & have1) == ~0ull;
@@ -310,30 +333,36 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
         if (!whole || ub + kFewKeys - 1 > all_hi || ub < all_lo) {
             const uint32_t bits[2] = {static_cast<uint32_t>(have0 >> (4 * g)), static_cast<uint32_t>(have1 >> (4 * g))};
 #pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int u = ub + 16 * b + 4 * g + i;
+                        if (!((bits[b] >> i) & 1) || u > hi[n] || u < lo[n]) s[n][b][i] = -INFINITY;
+                    }
+        }
+        uint4 p[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const float m2 = fmaxp(m[n], max_rows(max8(s[n])) * sp.sc2);
+            const float ref = m2 == -INFINITY ? 0.f : m2;
+            if (__ballot(m2 != m[n])) {
+                const float keep = __builtin_amdgcn_exp2f(m[n] - ref);
+                l[n] *= keep;
+#pragma unroll
+                for (int db = 0; db < DB; ++db) o[n][db] *= keep;
+            }
+            m[n] = m2;
+#pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int u = ub + 16 * b + 4 * g + i;
-                    if (!((bits[b] >> i) & 1) || u > hi || u < lo) s[b][i] = -INFINITY;
+                    s[n][b][i] = __builtin_amdgcn_exp2f(fmaf(s[n][b][i], sp.sc2, -ref));
+                    l[n] += s[n][b][i];
                 }
+            p[n] = pack8<T>(s[n]);
         }
-        const float m2 = fmaxp(m, max_rows(max8(s)) * sp.sc2);
-        const float ref = m2 == -INFINITY ? 0.f : m2;
-        if (__ballot(m2 != m)) {
-            const float keep = __builtin_amdgcn_exp2f(m - ref);
-            l *= keep;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) o[db] *= keep;
-        }
-        m = m2;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], sp.sc2, -ref));
-                l += s[b][i];
-            }
-        const uint4 p = pack8<T>(s);
         const int r0 = 4 * g + (col >> 2), r1 = 16 + r0;
         const int s0 = piece_swz<D>(r0), s1 = piece_swz<D>(r1);
 #pragma unroll
@@ -343,45 +372,42 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
             const T* const x1 = X + r1 * LD + ((pc ^ s1) << 3) + (col & 1) * 4;
             const uint2 lo2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x0));
             const uint2 hi2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x1));
-            o[db] = Mma<T>::run(make_uint4(lo2.x, lo2.y, hi2.x, hi2.y), p, o[db]);
+            const uint4 x = make_uint4(lo2.x, lo2.y, hi2.x, hi2.y);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) o[n][db] = Mma<T>::run(x, p[n], o[n][db]);
         }
     }
-    l = sum_rows(l);
-    // A probability of 0 times a value that is not finite: rows of the tile
-    // that do not attend to that key got NaN.  Redone key by key.
-    if (item_nonfinite(lane_sum(o, 0.f)) && !item_nonfinite(m) && !item_nonfinite(l)) {
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        for (int st = wave; st < steps; st += 4)
-            for (int e = 0; e < kFewKeys; ++e)
-                exact_key<T, D, DB, 16>(a, r, table, q, r.u_lo + st * kFewKeys + e, lo, hi, m, 4 * g, o);
-    }
     // the four waves' parts, through the LDS that held their values
-    float* const ow = reinterpret_cast<float*>(X);
+    float* const parts = reinterpret_cast<float*>(lds);  // [4][rows][D]
+    __syncthreads();
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
-        *reinterpret_cast<f32x4_t*>(ow + col * D + 16 * db + 4 * g) = o[db];
-    if (g == 0) {
-        ml[wave][col][0] = m;
-        ml[wave][col][1] = l;
+    for (int n = 0; n < NB; ++n) {
+        float* const ow = parts + (wave * kRowsOf + 16 * n + col) * D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(ow + 16 * db + 4 * g) = o[n][db];
+        l[n] = sum_rows(l[n]);
+        if (g == 0) {
+            ml[wave][16 * n + col][0] = m[n];
+            ml[wave][16 * n + col][1] = l[n];
+        }
     }
     lds_publish_barrier();
-    for (int e = threadIdx.x; e < kFewRows * (D / 4); e += kPagedThreads) {
+#pragma unroll 1
+    for (int e = threadIdx.x; e < r.rows * (D / 4); e += kPagedThreads) {
         const int rw = e / (D / 4), d = 4 * (e - rw * (D / 4));
-        if (rw >= r.rows) break;
         const float mt = fmaxp(fmaxp(ml[0][rw][0], ml[1][rw][0]), fmaxp(ml[2][rw][0], ml[3][rw][0]));
         const float ref = mt == -INFINITY ? 0.f : mt;
         float lt = 0.f;
         f32x4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            if (ml[w][rw][0] == -INFINITY && ml[w][rw][1] == 0.f) continue;
             const float wt = __builtin_amdgcn_exp2f(ml[w][rw][0] - ref);
             lt = fmaf(wt, ml[w][rw][1], lt);
-            x += wt * *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(vs[w]) + rw * D + d);
+            x += wt * *reinterpret_cast<const f32x4_t*>(parts + (w * kRowsOf + rw) * D + d);
         }
+        if (four_nonfinite(x) && !item_nonfinite(mt) && !item_nonfinite(lt)) x = exact_four<T, D>(a, r, rw, mt, d);
         if (r.split) {
-            const long long at = static_cast<long long>(r.index) * kFewRows + rw;
+            const long long at = static_cast<long long>(r.index) * kRowsOf + rw;
             *reinterpret_cast<f32x4_t*>(a.part + at * D + d) = x;
             if (d == 0) {
                 a.ml[2 * at] = mt;
@@ -452,14 +478,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
     constexpr int PR = D / 8;                        // pieces of a row
     constexpr int kLoads = kChunkKeys * PR / kPagedThreads;  // of a thread, keys and values each
     constexpr int kTile = kChunkKeys * LD;
-    __shared__ ShareScratch sh;
     __shared__ long long koff[2][kChunkKeys], voff[2][kChunkKeys];
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     T* const ks = reinterpret_cast<T*>(lds);
     T* const vs = ks + 2 * kTile;
     clear_padding<T>(a);
     Share r;
-    if (!find_share(a, sh, r)) return;
+    if (!find_share(a, r)) return;
     if (r.rows <= 0) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 31, h = lane >> 5;
@@ -651,24 +676,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
         int qi, qh;
         row_token(a, r.cls, r.h, r.row0 + rw, qi, qh);
         const float lt = l[b] + other_half(l[b]);
-        float total = 0.f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) total += o[b][t][i];
-        if (item_nonfinite(total) && !item_nonfinite(m[b]) && !item_nonfinite(lt)) {
-            // as in k_paged_few: 0 times a value that is not finite
-            f32x4_t e[D / 8];
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) e[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            const T* const q = static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
-            for (int u = r.u_lo; u <= r.u_hi; ++u)
-                exact_key<T, D, D / 8, 8>(a, r, table, q, u, lo[b], hi[b], m[b], 4 * h, e);
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[b][n / 4][4 * (n & 3) + i] = e[n][i];
-        }
         if (r.split) {
             const long long at = static_cast<long long>(r.index) * a.M + rw;
 #pragma unroll
@@ -680,16 +687,34 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
                 a.ml[2 * at] = m[b];
                 a.ml[2 * at + 1] = lt;
             }
-            continue;
         }
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
         T* const out = static_cast<T*>(a.out) + r.b * a.lo.b + qi * a.lo.s2 + qh * a.lo.h;
+        if (!r.split) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-            *reinterpret_cast<uint2*>(out + 8 * n + 4 * h) =
-                make_uint2(Mma<T>::pack(o[b][n / 4][4 * (n & 3)] * inv, o[b][n / 4][4 * (n & 3) + 1] * inv),
-                           Mma<T>::pack(o[b][n / 4][4 * (n & 3) + 2] * inv, o[b][n / 4][4 * (n & 3) + 3] * inv));
-        if (h == 0) a.lse[r.b * a.ll.b + qi * a.ll.s2 + qh * a.ll.h] = row_lse(m[b], lt);
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<uint2*>(out + 8 * n + 4 * h) =
+                    make_uint2(Mma<T>::pack(o[b][n / 4][4 * (n & 3)] * inv, o[b][n / 4][4 * (n & 3) + 1] * inv),
+                               Mma<T>::pack(o[b][n / 4][4 * (n & 3) + 2] * inv, o[b][n / 4][4 * (n & 3) + 3] * inv));
+            if (h == 0) a.lse[r.b * a.ll.b + qi * a.ll.s2 + qh * a.ll.h] = row_lse(m[b], lt);
+        }
+        float total = 0.f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) total += o[b][t][i];
+        if (item_nonfinite(total) && !item_nonfinite(m[b]) && !item_nonfinite(lt)) {
+            // written over, four head dims at a time
+#pragma unroll 1
+            for (int d = 4 * h; d < D; d += 8) {
+                const f32x4_t x = exact_four<T, D>(a, r, rw, m[b], d);
+                if (r.split)
+                    *reinterpret_cast<f32x4_t*>(a.part + (static_cast<long long>(r.index) * a.M + rw) * D + d) = x;
+                else
+                    *reinterpret_cast<uint2*>(out + d) = make_uint2(Mma<T>::pack(x[0] * inv, x[1] * inv),
+                                                                    Mma<T>::pack(x[2] * inv, x[3] * inv));
+            }
+        }
     }
 }
 
@@ -697,100 +722,92 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
 // joining parts
 // ---------------------------------------------------------------------------
 
-// Rows of tall tiles (few parts each): a group of lanes per row, the head dims
-// in fours, the parts in order.
-template <typename T>
-__global__ __launch_bounds__(kPagedThreads) void k_paged_join_rows(PagedArgs a) {
-    const int tile = blockIdx.x;
-    if (tile >= *a.count) return;
-    const PagedTile t = a.tiles[tile];
-    if (t.parts <= 1) return;
-    const int quads = a.Dv / 4, per = kPagedThreads / quads;
-    const int row = blockIdx.y * per + threadIdx.x / quads, d = 4 * (threadIdx.x % quads);
-    if (static_cast<int>(threadIdx.x) >= per * quads || row >= t.rows) return;
-    float m = -INFINITY;
-    for (int s = 0; s < t.parts; ++s)
-        m = fmaxp(m, a.ml[2 * ((static_cast<long long>(t.first) + static_cast<long long>(s) * t.step) * a.M + row)]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < t.parts; ++s) {
-        const long long at = (static_cast<long long>(t.first) + static_cast<long long>(s) * t.step) * a.M + row;
-        if (a.ml[2 * at] == -INFINITY && a.ml[2 * at + 1] == 0.f) continue;  // a part without keys
-        const float w = __builtin_amdgcn_exp2f(a.ml[2 * at] - ref);
-        l = fmaf(w, a.ml[2 * at + 1], l);
-        x += w * *reinterpret_cast<const f32x4_t*>(a.part + at * a.Dv + d);
-    }
-    int i, hq;
-    row_token(a, t.cls, t.h, t.row0 + row, i, hq);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* const out = static_cast<T*>(a.out) + t.b * a.lo.b + i * a.lo.s2 + hq * a.lo.h + d;
+constexpr int kJoinThreads = 1024;  // at most
+
+// A running (m, l, acc) and one more part's, m base 2; a part without keys
+// (m = -inf, l = 0, zeros) changes nothing.
+struct Joined {
+    float m = -INFINITY, l = 0.f;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    __device__ __forceinline__ void add(float m1, float l1, f32x4_t x) {
+        const float m2 = fmaxp(m, m1), ref = m2 == -INFINITY ? 0.f : m2;
+        const float w0 = __builtin_amdgcn_exp2f(m - ref), w1 = __builtin_amdgcn_exp2f(m1 - ref);
+        m = m2;
+        l = l * w0 + l1 * w1;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = from_f<T>(x[e] * inv);
-    if (d == 0) a.lse[t.b * a.ll.b + i * a.ll.s2 + hq * a.ll.h] = row_lse(m, l);
+        for (int e = 0; e < 4; ++e) acc[e] = acc[e] * w0 + x[e] * w1;
+    }
+};
+
+__device__ __forceinline__ f32x4_t four_of(const float* p, int d, int dim) {
+    if (dim % 4 == 0) return *reinterpret_cast<const f32x4_t*>(p + d);
+    f32x4_t x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = d + e < dim ? p[d + e] : 0.f;
+    return x;
 }
 
-// Low tiles with many parts: a workgroup per row, groups of lanes on
-// different parts, joined through LDS in a fixed order.
-template <typename T>
-__global__ __launch_bounds__(kPagedThreads) void k_paged_join(PagedArgs a) {
-    __shared__ float o[kPagedThreads][5];
-    const int tile = blockIdx.x;
-    if (tile >= *a.count) return;
-    const PagedTile t = a.tiles[tile];
-    const int row = blockIdx.y;
-    if (t.parts <= 1 || row >= t.rows) return;
-    const int tid = threadIdx.x;
-    float m = -INFINITY;
-    for (int s = tid; s < t.parts; s += kPagedThreads)
-        m = fmaxp(m, a.ml[2 * ((static_cast<long long>(t.first) + static_cast<long long>(s) * t.step) * a.M + row)]);
-    for (int x = 32; x >= 1; x >>= 1) m = fmaxp(m, __shfl_xor(m, x));
-    if ((tid & 63) == 0) o[tid >> 6][0] = m;
-    lds_publish_barrier();
-    m = fmaxp(fmaxp(o[0][0], o[1][0]), fmaxp(o[2][0], o[3][0]));
-    const float ref = m == -INFINITY ? 0.f : m;
-    __syncthreads();
-    // quads of head dims on consecutive threads, the parts over the rest
-    const int quads = (a.Dv + 3) / 4, groups = kPagedThreads / quads;
-    const int d = 4 * (tid % quads), g = tid / quads;
-    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    if (g < groups) {
-        for (int s = g; s < t.parts; s += groups) {
-            const long long at = (static_cast<long long>(t.first) + static_cast<long long>(s) * t.step) * a.M + row;
-            const float ms = a.ml[2 * at];
-            if (ms == -INFINITY && a.ml[2 * at + 1] == 0.f) continue;  // a part without keys
-            const float w = __builtin_amdgcn_exp2f(ms - ref);
-            l = fmaf(w, a.ml[2 * at + 1], l);
-            const float* const p = a.part + at * a.Dv + d;
-            if (a.Dv % 4 == 0) {
-                const float4 x = *reinterpret_cast<const float4*>(p);
-                acc[0] = fmaf(w, x.x, acc[0]);
-                acc[1] = fmaf(w, x.y, acc[1]);
-                acc[2] = fmaf(w, x.z, acc[2]);
-                acc[3] = fmaf(w, x.w, acc[3]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (d + e < a.Dv) acc[e] = fmaf(w, p[e], acc[e]);
-            }
+// Head dims in fours on consecutive lanes.  With WIDE, the groups of lanes
+// take different parts of one row (low tiles, many parts) and meet in LDS;
+// otherwise each takes a row of its own (tall tiles, few parts).  Either way
+// a thread joins its parts in order, so that results do not depend on which
+// workgroup ended first.  The parts come from other XCDs' writes, a trip to
+// memory each: the record is read beside the count, maxima beside sums and
+// results.
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(WIDE ? kJoinThreads : kPagedThreads) void k_paged_join(PagedArgs a) {
+    __shared__ float o[WIDE ? kJoinThreads : 1][7];
+    const int tid = threadIdx.x, quads = (a.Dv + 3) >> 2;
+    const int groups = static_cast<int>(blockDim.x) / quads;
+    const int g = tid / quads, d = 4 * (tid - g * quads);
+    const PagedTile t = a.tiles[blockIdx.x];
+    if (static_cast<int>(blockIdx.x) >= *a.count || t.parts <= 1) return;
+    const int row = WIDE ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y) * groups + g;
+    if (WIDE && row >= t.rows) return;
+    Joined j;
+    if (g < groups && row < t.rows) {
+#pragma unroll 8
+        for (int s = WIDE ? g : 0; s < t.parts; s += WIDE ? groups : 1) {
+            const long long at = (t.first + static_cast<long long>(s) * t.step) * a.M + row;
+            j.add(a.ml[2 * at], a.ml[2 * at + 1], four_of(a.part + at * a.Dv, d, a.Dv));
         }
     }
-    for (int e = 0; e < 4; ++e) o[tid][e] = acc[e];
-    o[tid][4] = l;
-    lds_publish_barrier();
-    if (g != 0) return;
-    for (int s = 1; s < groups; ++s) {
-        for (int e = 0; e < 4; ++e) acc[e] += o[s * quads + tid][e];
-        l += o[s * quads + tid][4];
+    if constexpr (WIDE) {
+        o[tid][0] = j.m;
+        o[tid][1] = j.l;
+        for (int e = 0; e < 4; ++e) o[tid][2 + e] = j.acc[e];
+        lds_publish_barrier();
+        // eight groups join theirs with every eighth one's, then the first
+        // joins the eight
+        if (g < 8) {
+            for (int s = g + 8; s < groups; s += 8) {
+                const float* const p = o[s * quads + tid - g * quads];
+                j.add(p[0], p[1], f32x4_t{p[2], p[3], p[4], p[5]});
+            }
+        }
+        __syncthreads();
+        if (g < 8) {
+            o[tid][0] = j.m;
+            o[tid][1] = j.l;
+            for (int e = 0; e < 4; ++e) o[tid][2 + e] = j.acc[e];
+        }
+        lds_publish_barrier();
+        if (g != 0) return;
+        for (int s = 1; s < 8 && s < groups; ++s) {
+            const float* const p = o[s * quads + tid];
+            j.add(p[0], p[1], f32x4_t{p[2], p[3], p[4], p[5]});
+        }
+    } else if (g >= groups || row >= t.rows) {
+        return;
     }
     int i, hq;
     row_token(a, t.cls, t.h, t.row0 + row, i, hq);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* const out = static_cast<T*>(a.out) + t.b * a.lo.b + i * a.lo.s2 + hq * a.lo.h;
+    const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+    T* const out = static_cast<T*>(a.out) + t.b * a.lo.b + i * a.lo.s2 + hq * a.lo.h + d;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (d + e < a.Dv) out[d + e] = from_f<T>(acc[e] * inv);
-    if (tid == 0) a.lse[t.b * a.ll.b + i * a.ll.s2 + hq * a.ll.h] = row_lse(m, l);
+        if (d + e < a.Dv) out[e] = from_f<T>(j.acc[e] * inv);
+    if (d == 0) a.lse[t.b * a.ll.b + i * a.ll.s2 + hq * a.ll.h] = row_lse(j.m, j.l);
 }
 
 // ---------------------------------------------------------------------------
@@ -803,21 +820,21 @@ constexpr int kTarget = 512;
 // Rows of a class from which the tall tiles are taken.
 constexpr int kChunkFrom = 64;
 
-// 32-query blocks of a wave: two where their accumulators leave two waves a
-// SIMD (see k_paged_chunk).
-constexpr int chunk_blocks(int dim) { return dim <= 64 ? 2 : 1; }
-
 enum PagedKind { kRows, kFew, kChunk };
 
 struct PagedPlan {
     PagedKind kind;
+    int blocks;  // query blocks of a wave
     int M, KT, least, xcd_run;
+    long long rows;   // of a class, at most
     long long tiles;  // tile slots of the batch
     int slots;        // of a (sequence, kv head)
     bool split;       // some tile's keys may be cut
     long long grid;
     size_t bytes;     // workspace
 };
+
+constexpr int exponent_of(int n) { return n <= 1 ? 0 : 1 + exponent_of(n / 2); }
 
 long long padded(long long bytes) { return (bytes + 255) & ~255ll; }
 
@@ -834,12 +851,18 @@ PagedPlan plan(const PagedCall& c) {
     const long long dil = c.dilation, classes = c.tokens < dil ? c.tokens : dil;
     const long long members = (c.tokens + dil - 1) / dil;
     p.kind = !on_mfma(c) ? kRows : members * rep < kChunkFrom ? kFew : kChunk;
+    const long long rows = p.rows = members * rep;
     if (p.kind == kChunk) {
-        p.M = 128 * chunk_blocks(c.dim_qk);
+        // 64 queries a wave where their accumulators leave two waves a SIMD
+        // and the tiles still fill the device
+        const long long tall = classes * ((rows + 255) / 256) * c.batch * c.heads_kv;
+        p.blocks = c.dim_qk <= 64 && tall >= kTarget ? 2 : 1;
+        p.M = 128 * p.blocks;
         p.KT = kChunkKeys;
-        p.least = 8;
+        p.least = 16;
     } else if (p.kind == kFew) {
-        p.M = kFewRows;
+        p.blocks = rows <= 16 ? 1 : rows <= 32 || c.dim_qk > 64 ? 2 : 4;
+        p.M = kFewRows * p.blocks;
         p.KT = 4 * kFewKeys;
         p.least = 2;
     } else {
@@ -874,25 +897,37 @@ PagedPlan plan(const PagedCall& c) {
     return p;
 }
 
-template <typename T>
-hipError_t launch_few(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
-    const dim3 grid(p.grid), block(kPagedThreads);
-    if (a.Dqk == 32)
-        NA_LAUNCH("na_paged_few", (k_paged_few<T, 32>), grid, block, 0, s, a);
-    else if (a.Dqk == 64)
-        NA_LAUNCH("na_paged_few", (k_paged_few<T, 64>), grid, block, 0, s, a);
-    else if (a.Dqk == 96)
-        NA_LAUNCH("na_paged_few", (k_paged_few<T, 96>), grid, block, 0, s, a);
-    else
-        NA_LAUNCH("na_paged_few", (k_paged_few<T, 128>), grid, block, 0, s, a);
-    return hipGetLastError();
+// LDS of k_paged_few: the waves' values, then their results.
+template <int D>
+constexpr size_t few_lds(int blocks) {
+    const size_t values = 4 * kFewKeys * row_elems<D>() * 2, results = 4 * kFewRows * blocks * D * sizeof(float);
+    return values > results ? values : results;
 }
 
 template <typename T, int D>
-hipError_t launch_chunk(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
-    constexpr int lds = 2 * 2 * kChunkKeys * row_elems<D>() * sizeof(T);
-    const auto kernel = k_paged_chunk<T, D, chunk_blocks(D)>;
-    NA_LAUNCH("na_paged_chunk", kernel, dim3(p.grid), dim3(kPagedThreads), lds, s, a);
+hipError_t launch_mfma(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+    const dim3 grid(p.grid), block(kPagedThreads);
+    if (p.kind == kChunk) {
+        constexpr int lds = 2 * 2 * kChunkKeys * row_elems<D>() * sizeof(T);
+        if constexpr (D <= 64) {
+            if (p.blocks == 2) {
+                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 2>), grid, block, lds, s, a);
+                return hipGetLastError();
+            }
+        }
+        NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1>), grid, block, lds, s, a);
+        return hipGetLastError();
+    }
+    if constexpr (D <= 64) {
+        if (p.blocks == 4) {
+            NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 4>), grid, block, few_lds<D>(4), s, a);
+            return hipGetLastError();
+        }
+    }
+    if (p.blocks == 2)
+        NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 2>), grid, block, few_lds<D>(2), s, a);
+    else
+        NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 1>), grid, block, few_lds<D>(1), s, a);
     return hipGetLastError();
 }
 
@@ -907,21 +942,24 @@ hipError_t launch_kind(const PagedArgs& a, const PagedPlan& p, bool vec, hipStre
             NA_LAUNCH("na_paged_rows", (k_paged_rows<T, 1>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
         e = hipGetLastError();
     } else if constexpr (!std::is_same<T, float>::value) {
-        if (p.kind == kFew) e = launch_few<T>(a, p, s);
-        else if (a.Dqk == 32) e = launch_chunk<T, 32>(a, p, s);
-        else if (a.Dqk == 64) e = launch_chunk<T, 64>(a, p, s);
-        else if (a.Dqk == 96) e = launch_chunk<T, 96>(a, p, s);
-        else e = launch_chunk<T, 128>(a, p, s);
+        if (a.Dqk == 32) e = launch_mfma<T, 32>(a, p, s);
+        else if (a.Dqk == 64) e = launch_mfma<T, 64>(a, p, s);
+        else if (a.Dqk == 96) e = launch_mfma<T, 96>(a, p, s);
+        else e = launch_mfma<T, 128>(a, p, s);
     }
     if (e != hipSuccess || !p.split) return e;
+    const unsigned tiles = static_cast<unsigned>(p.tiles < kTarget ? p.tiles : kTarget);
+    const unsigned rows = static_cast<unsigned>(std::min<long long>(p.M, p.rows));
     if (p.kind == kChunk) {
-        const int per = kPagedThreads / (a.Dv / 4);
-        NA_LAUNCH("na_paged_join", (k_paged_join_rows<T>),
-                  dim3(p.tiles < kTarget ? p.tiles : kTarget, (p.M + per - 1) / per), dim3(kPagedThreads), 0, s, a);
-        return hipGetLastError();
+        const unsigned groups = kPagedThreads / (a.Dv / 4);
+        NA_LAUNCH("na_paged_join", (k_paged_join<T, false>), dim3(tiles, (rows + groups - 1) / groups),
+                  dim3(kPagedThreads), 0, s, a);
+    } else {
+        // parts per tile go as one over the tiles: enough groups of lanes
+        // that each joins a handful
+        const int threads = tiles <= 16 ? kJoinThreads : kPagedThreads;
+        NA_LAUNCH("na_paged_join", (k_paged_join<T, true>), dim3(tiles, rows), dim3(threads), 0, s, a);
     }
-    NA_LAUNCH("na_paged_join", (k_paged_join<T>), dim3(p.tiles < kTarget ? p.tiles : kTarget, p.M),
-              dim3(kPagedThreads), 0, s, a);
     return hipGetLastError();
 }
 
@@ -959,7 +997,8 @@ hipError_t paged_forward(const PagedCall& c, hipStream_t s) {
     a.lens = c.cache.lens;
     a.news = c.cache.news;
     a.table_stride = c.cache.table_stride;
-    a.width = c.cache.width;
+    const long long cap = static_cast<long long>(c.cache.width) * c.cache.page_size;
+    a.cap = static_cast<int>(std::min<long long>(cap, 0x7fffffff));
     a.pages = c.cache.pages;
     a.page_size = c.cache.page_size;
     a.fpage = make_fastdiv(a.page_size);
@@ -971,15 +1010,18 @@ hipError_t paged_forward(const PagedCall& c, hipStream_t s) {
     a.Dqk = c.dim_qk;
     a.Dv = c.cache.dim_v;
     a.frep = make_fastdiv(a.rep);
+    a.flen = make_fastdiv(a.L);
+    a.fdv = make_fastdiv(a.Dv);
     a.K = c.kernel;
     a.dil = c.dilation;
     a.fdil = make_fastdiv(a.dil);
     a.scale = c.scale;
     a.M = p.M;
-    a.KT = p.KT;
+    a.log_m = exponent_of(p.M);
+    a.log_kt = exponent_of(p.KT);
     a.tile_slots = p.slots;
     a.direct = p.split ? 0 : 1;
-    a.target = kTarget;
+    a.log_target = exponent_of(kTarget);
     a.least = p.least;
     a.xcd_run = p.xcd_run;
     a.frun = make_fastdiv(imax(p.xcd_run, 1));
