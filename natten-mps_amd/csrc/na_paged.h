@@ -47,6 +47,7 @@ struct PagedArgs {
     int least;             // key blocks of a chunk at least
     int xcd_run;           // consecutive shares of one XCD (0: as dealt)
     FastDiv fslots, fkv, frun;
+    int per_wave;          // tokens of the batch that a wave looks at for padding
     // split tiles: header (count of tiles), a record per tile, m and l, O
     int* count;
     struct PagedTile* tiles;

@@ -23,22 +23,31 @@ namespace na {
 
 namespace {
 
-// Rows of padding tokens: zeros, and -inf.  The workgroups of the grid share
-// the batch's tokens.
+// Rows of padding tokens: zeros, and -inf.  The grid's waves share the batch's
+// tokens evenly, a lane looks whether one is padding, then the wave clears
+// those that are.
 template <typename T>
 __device__ __forceinline__ void clear_padding(const PagedArgs& a) {
     if (!a.news) return;
-    const int tokens = a.B * a.L;
-    for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
-        const int b = fdiv(t, a.flen), i = t - b * a.L;
-        if (i < a.news[b]) continue;
-        T* const o = static_cast<T*>(a.out) + b * a.lo.b + i * a.lo.s2;
-        for (int e = threadIdx.x; e < a.Hq * a.Dv; e += kPagedThreads) {
-            const int h = fdiv(e, a.fdv);
-            o[h * a.lo.h + (e - h * a.Dv)] = from_f<T>(0.f);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kPagedThreads / 64) + (threadIdx.x >> 6));
+    const int first = wave * a.per_wave, end = imin(first + a.per_wave, a.B * a.L);
+    for (int t0 = first; t0 < end; t0 += 64) {
+        const int t = t0 + lane;
+        bool pad = false;
+        if (t < end) {
+            const int b = fdiv(t, a.flen);
+            pad = t - b * a.L >= a.news[b];
         }
-        for (int h = threadIdx.x; h < a.Hq; h += kPagedThreads)
-            a.lse[b * a.ll.b + i * a.ll.s2 + h * a.ll.h] = -INFINITY;
+        for (unsigned long long left = __ballot(pad); left; left &= left - 1) {
+            const int x = t0 + __ffsll(left) - 1, b = fdiv(x, a.flen), i = x - b * a.L;
+            T* const o = static_cast<T*>(a.out) + b * a.lo.b + i * a.lo.s2;
+            for (int e = lane; e < a.Hq * a.Dv; e += 64) {
+                const int h = fdiv(e, a.fdv);
+                o[h * a.lo.h + (e - h * a.Dv)] = from_f<T>(0.f);
+            }
+            for (int h = lane; h < a.Hq; h += 64) a.lse[b * a.ll.b + i * a.ll.s2 + h * a.ll.h] = -INFINITY;
+        }
     }
 }
 
@@ -158,6 +167,12 @@ __device__ __forceinline__ int piece_swz(int row) {
     else return (((row >> 2) & 1) << 1) | odd;
 }
 
+// A row's running maximum is raised, and what was summed scaled down, only
+// where the scores pass it by this many powers of two: early keys seldom hold
+// the maximum, and exponentials up to 2^8 lose nothing (fp16 holds 2^15, a
+// sum in fp32 of 2^31 of them is far from its limit).
+constexpr float kSlack = 8.f;
+
 // The scale's sign goes into the queries (exact), a scale of zero makes them
 // zero, so that scores times `sc2` > 0 order as the logits do.
 struct ScaleParts {
@@ -224,7 +239,7 @@ __device__ __forceinline__ bool four_nonfinite(f32x4_t x) { return item_nonfinit
 constexpr int kFewRows = 16, kFewKeys = 32;
 
 template <typename T, int D, int NB>
-__global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
+__global__ __launch_bounds__(kPagedThreads, NB > 1 ? 2 : D > 64 ? 3 : 4) void k_paged_few(PagedArgs a) {
     constexpr int C = D / 32, LD = row_elems<D>(), DB = D / 16;
     constexpr int kRowsOf = kFewRows * NB;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
@@ -238,7 +253,8 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
     const ScaleParts sp = scale_parts(a.scale);
     // queries, their windows, and what all rows of the tile see
     uint4 qf[NB][C];
-    int hi[NB], lo[NB];
+    int hi[NB];
+    const uint32_t reach = a.K ? a.K - 1 : 0x7fffffffu;  // keys behind a query's own
     auto query = [&](int n) {
         int qi, qh;
         row_token(a, r.cls, r.h, r.row0 + imin(16 * n + col, r.rows - 1), qi, qh);
@@ -250,7 +266,6 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) qf[n][c] = scaled(*reinterpret_cast<const uint4*>(q + 32 * c + 8 * g), sp);
         hi[n] = r.w0 + fdiv(r.row0 + imin(16 * n + col, r.rows - 1), a.frep);
-        lo[n] = a.K ? hi[n] - a.K + 1 : 0;
     }
     const int all_hi = imin(r.w0 + fdiv(r.row0, a.frep), r.u_hi);
     const int all_lo = a.K ? r.w0 + fdiv(r.row0 + r.rows - 1, a.frep) - a.K + 1 : 0;
@@ -333,27 +348,30 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_few(PagedArgs a) {
         if (!whole || ub + kFewKeys - 1 > all_hi || ub < all_lo) {
             const uint32_t bits[2] = {static_cast<uint32_t>(have0 >> (4 * g)), static_cast<uint32_t>(have1 >> (4 * g))};
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+            for (int n = 0; n < NB; ++n) {
+                // keys ahead of the query count as far behind it
+                const uint32_t back = static_cast<uint32_t>(hi[n] - ub - 4 * g);
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int u = ub + 16 * b + 4 * g + i;
-                        if (!((bits[b] >> i) & 1) || u > hi[n] || u < lo[n]) s[n][b][i] = -INFINITY;
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        if (back - (16 * b + i) > reach || !((bits[b] >> i) & 1)) s[n][b][i] = -INFINITY;
+            }
         }
         uint4 p[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            const float m2 = fmaxp(m[n], max_rows(max8(s[n])) * sp.sc2);
-            const float ref = m2 == -INFINITY ? 0.f : m2;
-            if (__ballot(m2 != m[n])) {
-                const float keep = __builtin_amdgcn_exp2f(m[n] - ref);
+            const float top = max_rows(max8(s[n])) * sp.sc2;
+            const bool raise = top > m[n] + kSlack;
+            if (__ballot(raise)) {
+                const float m2 = raise ? top : m[n];
+                const float keep = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - m2);
+                m[n] = m2;
                 l[n] *= keep;
 #pragma unroll
                 for (int db = 0; db < DB; ++db) o[n][db] *= keep;
             }
-            m[n] = m2;
+            const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -472,13 +490,14 @@ __device__ __forceinline__ float other_half(float v) {
 // i % 4, and the values' operand is read (transposed) in that order.
 constexpr int kChunkKeys = 64;
 
-template <typename T, int D, int QB>
+template <typename T, int D, int QB, int SUB>
 __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
     constexpr int C = D / 16, LD = row_elems<D>(), DT = D / 32;
     constexpr int PR = D / 8;                        // pieces of a row
-    constexpr int kLoads = kChunkKeys * PR / kPagedThreads;  // of a thread, keys and values each
-    constexpr int kTile = kChunkKeys * LD;
-    __shared__ long long koff[2][kChunkKeys], voff[2][kChunkKeys];
+    constexpr int KT = kChunkKeys * SUB;             // keys staged at once
+    constexpr int kLoads = KT * PR / kPagedThreads;  // of a thread, keys and values each
+    constexpr int kTile = KT * LD;
+    __shared__ long long koff[2][KT], voff[2][KT];
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     T* const ks = reinterpret_cast<T*>(lds);
     T* const vs = ks + 2 * kTile;
@@ -494,7 +513,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
     const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh;
     const int wrow = 32 * QB * wave;  // the wave's first row in the tile
     uint4 qf[QB][C];
-    int hi[QB], lo[QB];
+    int hi[QB];
+    const uint32_t reach = a.K ? a.K - 1 : 0x7fffffffu;  // keys behind a query's own
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
         const int row = r.row0 + imin(wrow + 32 * b + col, r.rows - 1);
@@ -504,24 +524,25 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) qf[b][c] = scaled(*reinterpret_cast<const uint4*>(q + 16 * c + 8 * h), sp);
         hi[b] = r.w0 + fdiv(row, a.frep);
-        lo[b] = a.K ? hi[b] - a.K + 1 : 0;
     }
     // what some and what all rows of the wave see
     const int wf = r.w0 + fdiv(r.row0 + imin(wrow, r.rows - 1), a.frep);
     const int wl = r.w0 + fdiv(r.row0 + imin(wrow + 32 * QB, r.rows) - 1, a.frep);
     const int some_lo = a.K ? wf - a.K + 1 : 0, all_lo = a.K ? wl - a.K + 1 : 0;
     const bool idle = wrow >= r.rows;
-    const int steps = (r.u_hi - r.u_lo + kChunkKeys) / kChunkKeys;
+    const int steps = (r.u_hi - r.u_lo + KT) / KT;
 
-    // Offsets of tile st's keys by lane, -1 where no page holds one; the page
-    // number is asked for well before.
+    // Offsets of stage st's keys, -1 where no page holds one: SUB waves, 64
+    // keys each, other waves for other stages.  The page number is asked for
+    // well before it is used.
+    const int part = SUB == 1 ? 0 : wave & (SUB - 1);
     int page = -1, slot = 0;
     auto ask = [&](int st) {
-        if (!key_at(a, table, r.c, r.u_lo + st * kChunkKeys + lane, r.u_hi, page, slot)) page = -1;
+        if (!key_at(a, table, r.c, r.u_lo + st * KT + 64 * part + lane, r.u_hi, page, slot)) page = -1;
     };
     auto locate = [&](int st) {
-        koff[st & 1][lane] = page >= 0 ? page * a.kp + slot * a.ks : -1;
-        voff[st & 1][lane] = page >= 0 ? page * a.vp + slot * a.vs : -1;
+        koff[st & 1][64 * part + lane] = page >= 0 ? page * a.kp + slot * a.ks : -1;
+        voff[st & 1][64 * part + lane] = page >= 0 ? page * a.vp + slot * a.vs : -1;
     };
     uint4 kx[kLoads], vx[kLoads];
     auto load = [&](int st) {
@@ -557,29 +578,33 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[b][t][i] = 0.f;
     }
-    unsigned long long have = 0;
+    unsigned long long have[SUB] = {};
     if (steps > 0) {
-        if (wave < 2 && wave < steps) {
-            ask(wave);
-            locate(wave);
+        if (wave < 2 * SUB && wave / SUB < steps) {
+            ask(wave / SUB);
+            locate(wave / SUB);
         }
         lds_publish_barrier();
-        have = __ballot(koff[0][lane] >= 0);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) have[u] = __ballot(koff[0][64 * u + lane] >= 0);
         load(0);
         store(0);
         lds_publish_barrier();
     }
     for (int st = 0; st < steps; ++st) {
-        const int ub = r.u_lo + st * kChunkKeys;
-        unsigned long long have_next = 0;
-        const bool asks = st + 2 < steps && wave == (st & 3);
+        unsigned long long have_next[SUB] = {};
+        const bool asks = st + 2 < steps && wave / SUB == (st & (4 / SUB - 1));
         if (asks) ask(st + 2);
         if (st + 1 < steps) {
-            have_next = __ballot(koff[(st + 1) & 1][lane] >= 0);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) have_next[u] = __ballot(koff[(st + 1) & 1][64 * u + lane] >= 0);
             load(st + 1);
         }
-        const T* const K = ks + (st & 1) * kTile;
-        const T* const V = vs + (st & 1) * kTile;
+#pragma unroll
+        for (int sub = 0; sub < SUB; ++sub) {
+        const int ub = r.u_lo + st * KT + sub * kChunkKeys;
+        const T* const K = ks + (st & 1) * kTile + sub * kChunkKeys * LD;
+        const T* const V = vs + (st & 1) * kTile + sub * kChunkKeys * LD;
         if (!idle && ub <= wl && ub + kChunkKeys - 1 >= some_lo) {
             f32x16_t s[QB][2];
 #pragma unroll
@@ -597,18 +622,28 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
                     for (int b = 0; b < QB; ++b) s[b][kb2] = mma32<T>(kf, qf[b][c], s[b][kb2]);
                 }
             }
-            if (have != ~0ull || ub + kChunkKeys - 1 > wf || ub < all_lo) {
+            if (have[sub] != ~0ull || ub + kChunkKeys - 1 > wf || ub < all_lo) {
 #pragma unroll
-                for (int b = 0; b < QB; ++b)
+                for (int b = 0; b < QB; ++b) {
+                    // keys ahead of the query count as far behind it
+                    const uint32_t back = static_cast<uint32_t>(hi[b] - ub - 4 * h);
+#pragma unroll
+                    for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (back - (32 * kb2 + 8 * (i / 4) + (i & 3)) > reach) s[b][kb2][i] = -INFINITY;
+                }
+                if (have[sub] != ~0ull) {
 #pragma unroll
                     for (int kb2 = 0; kb2 < 2; ++kb2) {
-                        const uint32_t bits = static_cast<uint32_t>(have >> (32 * kb2)) >> (4 * h);
+                        const uint32_t bits = static_cast<uint32_t>(have[sub] >> (32 * kb2)) >> (4 * h);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int k = 8 * (i / 4) + (i & 3), u = ub + 32 * kb2 + 4 * h + k;
-                            if (!((bits >> k) & 1) || u > hi[b] || u < lo[b]) s[b][kb2][i] = -INFINITY;
-                        }
+                        for (int i = 0; i < 16; ++i)
+#pragma unroll
+                            for (int b = 0; b < QB; ++b)
+                                if (!((bits >> (8 * (i / 4) + (i & 3))) & 1)) s[b][kb2][i] = -INFINITY;
                     }
+                }
             }
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
@@ -616,14 +651,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
 #pragma unroll
                 for (int i = 1; i < 16; ++i) top = fmaxp(top, fmaxp(s[b][0][i], s[b][1][i]));
                 top = fmaxp(top, other_half(top)) * sp.sc2;
-                const float m2 = fmaxp(m[b], top), ref = m2 == -INFINITY ? 0.f : m2;
-                if (__ballot(m2 != m[b])) {
-                    const float keep = __builtin_amdgcn_exp2f(m[b] - ref);
+                const bool raise = top > m[b] + kSlack;
+                if (__ballot(raise)) {
+                    const float m2 = raise ? top : m[b];
+                    const float keep = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[b] - m2);
+                    m[b] = m2;
                     l[b] *= keep;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) o[b][t] *= keep;
                 }
-                m[b] = m2;
+                const float ref = m[b] == -INFINITY ? 0.f : m[b];
                 float sum = 0.f;
 #pragma unroll
                 for (int kb2 = 0; kb2 < 2; ++kb2)
@@ -661,7 +698,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
                 }
             }
         }
-        have = have_next;
+        }
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) have[u] = have_next[u];
         if (st + 1 < steps) {
             store(st + 1);
             // the offsets of tile st + 2 replace those of tile st
@@ -910,12 +949,13 @@ hipError_t launch_mfma(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
     if (p.kind == kChunk) {
         constexpr int lds = 2 * 2 * kChunkKeys * row_elems<D>() * sizeof(T);
         if constexpr (D <= 64) {
-            if (p.blocks == 2) {
-                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 2>), grid, block, lds, s, a);
-                return hipGetLastError();
-            }
+            if (p.blocks == 2)
+                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 2, 1>), grid, block, lds, s, a);
+            else
+                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 2>), grid, block, 2 * lds, s, a);
+        } else {
+            NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 1>), grid, block, lds, s, a);
         }
-        NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1>), grid, block, lds, s, a);
         return hipGetLastError();
     }
     if constexpr (D <= 64) {
@@ -1024,6 +1064,8 @@ hipError_t paged_forward(const PagedCall& c, hipStream_t s) {
     a.log_target = exponent_of(kTarget);
     a.least = p.least;
     a.xcd_run = p.xcd_run;
+    const long long waves = p.grid * (kPagedThreads / 64);
+    a.per_wave = static_cast<int>((static_cast<long long>(a.B) * a.L + waves - 1) / waves);
     a.frun = make_fastdiv(imax(p.xcd_run, 1));
     a.fslots = make_fastdiv(p.slots);
     a.fkv = make_fastdiv(a.Hkv);
