@@ -448,6 +448,8 @@ __global__ __launch_bounds__(kPagedThreads, NB > 1 ? 2 : D > 64 ? 3 : 4) void k_
 // ---------------------------------------------------------------------------
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef long long i64x2_t __attribute__((ext_vector_type(2)));
 
 template <typename T>
 __device__ __forceinline__ f32x16_t mma32(uint4 a, uint4 b, f32x16_t c) {
@@ -490,14 +492,14 @@ __device__ __forceinline__ float other_half(float v) {
 // i % 4, and the values' operand is read (transposed) in that order.
 constexpr int kChunkKeys = 64;
 
-template <typename T, int D, int QB, int SUB>
-__global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
+template <typename T, int D, int QB, int DEPTH>
+__global__ __launch_bounds__(kPagedThreads, DEPTH == 2 ? 3 : 2) void k_paged_chunk(PagedArgs a) {
     constexpr int C = D / 16, LD = row_elems<D>(), DT = D / 32;
-    constexpr int PR = D / 8;                        // pieces of a row
-    constexpr int KT = kChunkKeys * SUB;             // keys staged at once
-    constexpr int kLoads = KT * PR / kPagedThreads;  // of a thread, keys and values each
-    constexpr int kTile = KT * LD;
-    __shared__ long long koff[2][KT], voff[2][KT];
+    constexpr int PR = D / 8;                                // pieces of a row
+    constexpr int kLoads = kChunkKeys * PR / kPagedThreads;  // of a thread, keys and values each
+    constexpr int kTile = kChunkKeys * LD, kOffs = DEPTH + 1;
+    __shared__ i64x2_t off[kOffs][kChunkKeys];  // of a key's row in the key and value pages
+    __shared__ int live[kOffs][kChunkKeys];
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     T* const ks = reinterpret_cast<T*>(lds);
     T* const vs = ks + 2 * kTile;
@@ -530,42 +532,65 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
     const int wl = r.w0 + fdiv(r.row0 + imin(wrow + 32 * QB, r.rows) - 1, a.frep);
     const int some_lo = a.K ? wf - a.K + 1 : 0, all_lo = a.K ? wl - a.K + 1 : 0;
     const bool idle = wrow >= r.rows;
-    const int steps = (r.u_hi - r.u_lo + KT) / KT;
+    const int steps = (r.u_hi - r.u_lo + kChunkKeys) / kChunkKeys;
 
-    // Offsets of stage st's keys, -1 where no page holds one: SUB waves, 64
-    // keys each, other waves for other stages.  The page number is asked for
-    // well before it is used.
-    const int part = SUB == 1 ? 0 : wave & (SUB - 1);
-    int page = -1, slot = 0;
+    // Where tile st's keys are (the pool's first slot where no page holds one:
+    // live 0), by the waves in turn.  The page number is asked for well before
+    // it is used, the offsets lie in LDS a step before they are.
+    int page = 0, slot = 0;
+    bool in = false;
     auto ask = [&](int st) {
-        if (!key_at(a, table, r.c, r.u_lo + st * KT + 64 * part + lane, r.u_hi, page, slot)) page = -1;
+        const int u = r.u_lo + st * kChunkKeys + lane;
+        in = u <= r.u_hi;
+        const int j = r.c + imin(u, r.u_hi) * a.dil, pg = fdiv(j, a.fpage);
+        slot = j - pg * a.page_size;
+        page = table[pg];
     };
     auto locate = [&](int st) {
-        koff[st & 1][64 * part + lane] = page >= 0 ? page * a.kp + slot * a.ks : -1;
-        voff[st & 1][64 * part + lane] = page >= 0 ? page * a.vp + slot * a.vs : -1;
+        const bool ok = in && page >= 0 && page < a.pages;
+        const int pg = ok ? page : 0, sl = ok ? slot : 0;
+        off[st % kOffs][lane] = i64x2_t{pg * a.kp + sl * a.ks, pg * a.vp + sl * a.vs};
+        live[st % kOffs][lane] = ok;
     };
-    uint4 kx[kLoads], vx[kLoads];
-    auto load = [&](int st) {
+    auto row_of = [&](int i) { return (tid + i * kPagedThreads) / PR; };
+    auto piece_of = [&](int i) { return (tid + i * kPagedThreads) % PR; };
+    auto find = [&](int st, i64x2_t (&x)[kLoads]) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) x[i] = off[st % kOffs][row_of(i)];
+    };
+    auto load = [&](const i64x2_t (&x)[kLoads], u32x4_t (&kv)[2][kLoads]) {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int rw = (tid + i * kPagedThreads) / PR, lpc = (tid + i * kPagedThreads) % PR;
-            const long long ko = koff[st & 1][rw], vo = voff[st & 1][rw];
-            kx[i] = make_uint4(0, 0, 0, 0);
-            vx[i] = make_uint4(0, 0, 0, 0);
-            if (ko >= 0) {
-                kx[i] = *reinterpret_cast<const uint4*>(kb + ko + 8 * lpc);
-                vx[i] = *reinterpret_cast<const uint4*>(vb + vo + 8 * lpc);
-            }
+            kv[0][i] = *reinterpret_cast<const u32x4_t*>(kb + 8 * piece_of(i) + x[i].x);
+            kv[1][i] = *reinterpret_cast<const u32x4_t*>(vb + 8 * piece_of(i) + x[i].y);
         }
     };
-    auto store = [&](int st) {
+    auto store = [&](int st, bool whole, const u32x4_t (&kv)[2][kLoads]) {
+        // values that are not there must not be: 0 times them is in the sum
+        uint32_t keep[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) keep[i] = 0xffffffffu;
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) keep[i] = live[st % kOffs][row_of(i)] ? 0xffffffffu : 0u;
+        }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int rw = (tid + i * kPagedThreads) / PR, lpc = (tid + i * kPagedThreads) % PR;
-            *reinterpret_cast<uint4*>(ks + (st & 1) * kTile + rw * LD + ((lpc ^ key_swz<LD>(rw)) << 3)) = kx[i];
-            *reinterpret_cast<uint4*>(vs + (st & 1) * kTile + rw * LD + ((lpc ^ value_swz<LD>(rw)) << 3)) = vx[i];
+            const int rw = row_of(i), pc = piece_of(i);
+            *reinterpret_cast<u32x4_t*>(ks + (st & 1) * kTile + rw * LD + ((pc ^ key_swz<LD>(rw)) << 3)) = kv[0][i];
+            *reinterpret_cast<u32x4_t*>(vs + (st & 1) * kTile + rw * LD + ((pc ^ value_swz<LD>(rw)) << 3)) =
+                kv[1][i] & keep[i];
         }
     };
+    auto present = [&](int st) { return __ballot(live[st % kOffs][lane] != 0); };
+    // A lane's places in a tile's rows: the swizzles repeat every 16 (keys)
+    // and 8 (values) rows, so the rest of an address is constant.
+    int kat[C], vat[DT];
+#pragma unroll
+    for (int c = 0; c < C; ++c) kat[c] = col * LD + (((2 * c + h) ^ key_swz<LD>(col)) << 3);
+    const int vr = 4 * h + ((lane & 15) >> 2), vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) vat[t] = vr * LD + (((4 * t + vc) ^ value_swz<LD>(vr)) << 3) + (lane & 1) * 4;
 
     float m[QB], l[QB];
     f32x16_t o[QB][DT];
@@ -578,51 +603,64 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[b][t][i] = 0.f;
     }
-    unsigned long long have[SUB] = {};
+    unsigned long long have = 0;
+    u32x4_t buf[DEPTH][2][kLoads];
     if (steps > 0) {
-        if (wave < 2 * SUB && wave / SUB < steps) {
-            ask(wave / SUB);
-            locate(wave / SUB);
+        // tile 0 into LDS; with two in flight, tile 1 on its way
+        if (wave < kOffs && wave < steps) {
+            ask(wave);
+            locate(wave);
         }
         lds_publish_barrier();
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) have[u] = __ballot(koff[0][64 * u + lane] >= 0);
-        load(0);
-        store(0);
+        have = present(0);
+        i64x2_t x[kLoads];
+        find(0, x);
+        load(x, buf[0]);
+        store(0, false, buf[0]);
+        if (DEPTH == 2 && steps > 1) {
+            find(1, x);
+            load(x, buf[0]);
+        }
         lds_publish_barrier();
     }
-    for (int st = 0; st < steps; ++st) {
-        unsigned long long have_next[SUB] = {};
-        const bool asks = st + 2 < steps && wave / SUB == (st & (4 / SUB - 1));
-        if (asks) ask(st + 2);
-        if (st + 1 < steps) {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) have_next[u] = __ballot(koff[(st + 1) & 1][64 * u + lane] >= 0);
-            load(st + 1);
-        }
-#pragma unroll
-        for (int sub = 0; sub < SUB; ++sub) {
-        const int ub = r.u_lo + st * KT + sub * kChunkKeys;
-        const T* const K = ks + (st & 1) * kTile + sub * kChunkKeys * LD;
-        const T* const V = vs + (st & 1) * kTile + sub * kChunkKeys * LD;
-        if (!idle && ub <= wl && ub + kChunkKeys - 1 >= some_lo) {
-            f32x16_t s[QB][2];
+
+    // One tile: `next` goes into LDS at its end (with DEPTH 1, loaded at its
+    // start), `after` is loaded at its start with DEPTH 2.
+    auto step = [&](int st, u32x4_t (&next)[2][kLoads], u32x4_t (&after)[2][kLoads]) {
+        const bool more = st + 1 < steps, loads = st + DEPTH < steps;
+        const bool asks = st + kOffs < steps && wave == (st & 3);
+        unsigned long long have_next = 0;
+        i64x2_t x[kLoads];
+        if (loads) find(st + DEPTH, x);
+        if (more) have_next = present(st + 1);
+        const int ub = r.u_lo + st * kChunkKeys;
+        const T* const K = ks + (st & 1) * kTile;
+        const T* const V = vs + (st & 1) * kTile;
+        const bool busy = !idle && ub <= wl && ub + kChunkKeys - 1 >= some_lo;
+        f32x16_t s[QB][2];
+        if (busy) {
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kb2 = 0; kb2 < 2; ++kb2) {
-                const int rw = 32 * kb2 + col;
 #pragma unroll
                 for (int b = 0; b < QB; ++b)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[b][kb2][i] = 0.f;
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const uint4 kf =
-                        *reinterpret_cast<const uint4*>(K + rw * LD + (((2 * c + h) ^ key_swz<LD>(rw)) << 3));
+                    const uint4 kf = *reinterpret_cast<const uint4*>(K + kat[c] + 32 * kb2 * LD);
 #pragma unroll
                     for (int b = 0; b < QB; ++b) s[b][kb2] = mma32<T>(kf, qf[b][c], s[b][kb2]);
                 }
             }
-            if (have[sub] != ~0ull || ub + kChunkKeys - 1 > wf || ub < all_lo) {
+            __builtin_amdgcn_s_setprio(0);
+        }
+        // loads go out behind the scores' products, the page number first:
+        // waiting for it then waits for no keys
+        if (asks) ask(st + kOffs);
+        if (loads) load(x, DEPTH == 2 ? after : next);
+        if (busy) {
+            if (have != ~0ull || ub + kChunkKeys - 1 > wf || ub < all_lo) {
 #pragma unroll
                 for (int b = 0; b < QB; ++b) {
                     // keys ahead of the query count as far behind it
@@ -633,10 +671,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
                         for (int i = 0; i < 16; ++i)
                             if (back - (32 * kb2 + 8 * (i / 4) + (i & 3)) > reach) s[b][kb2][i] = -INFINITY;
                 }
-                if (have[sub] != ~0ull) {
+                if (have != ~0ull) {
 #pragma unroll
                     for (int kb2 = 0; kb2 < 2; ++kb2) {
-                        const uint32_t bits = static_cast<uint32_t>(have[sub] >> (32 * kb2)) >> (4 * h);
+                        const uint32_t bits = static_cast<uint32_t>(have >> (32 * kb2)) >> (4 * h);
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
 #pragma unroll
@@ -645,6 +683,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
                     }
                 }
             }
+            float ref[QB];
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
                 float top = fmaxp(s[b][0][0], s[b][1][0]);
@@ -660,53 +699,50 @@ __global__ __launch_bounds__(kPagedThreads, 2) void k_paged_chunk(PagedArgs a) {
 #pragma unroll
                     for (int t = 0; t < DT; ++t) o[b][t] *= keep;
                 }
-                const float ref = m[b] == -INFINITY ? 0.f : m[b];
-                float sum = 0.f;
-#pragma unroll
-                for (int kb2 = 0; kb2 < 2; ++kb2)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[b][kb2][i] = __builtin_amdgcn_exp2f(fmaf(s[b][kb2][i], sp.sc2, -ref));
-                        sum += s[b][kb2][i];
-                    }
-                l[b] += sum;
+                ref[b] = m[b] == -INFINITY ? 0.f : m[b];
             }
-            // 16 keys at a time
-            const int vr = 4 * h + ((lane & 15) >> 2), vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            // 16 keys at a time: the next ones' exponentials beside these
+            // ones' products
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
                 uint4 p[QB];
 #pragma unroll
                 for (int b = 0; b < QB; ++b) {
-                    const f32x16_t& x = s[b][kk >> 1];
-                    const int i0 = 8 * (kk & 1);
-                    p[b] = make_uint4(Mma<T>::pack(x[i0], x[i0 + 1]), Mma<T>::pack(x[i0 + 2], x[i0 + 3]),
-                                      Mma<T>::pack(x[i0 + 4], x[i0 + 5]), Mma<T>::pack(x[i0 + 6], x[i0 + 7]));
+                    float e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        e[i] = __builtin_amdgcn_exp2f(fmaf(s[b][kk >> 1][8 * (kk & 1) + i], sp.sc2, -ref[b]));
+                        l[b] += e[i];
+                    }
+                    p[b] = make_uint4(Mma<T>::pack(e[0], e[1]), Mma<T>::pack(e[2], e[3]), Mma<T>::pack(e[4], e[5]),
+                                      Mma<T>::pack(e[6], e[7]));
                 }
-                const int r0 = 16 * kk + vr, r1 = r0 + 8;
-                const T* const x0 = V + r0 * LD + (lane & 1) * 4;
-                const T* const x1 = V + r1 * LD + (lane & 1) * 4;
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    const uint2 lo2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_i16x4_t*)(x0 + (((4 * t + vc) ^ value_swz<LD>(r0)) << 3))));
-                    const uint2 hi2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_i16x4_t*)(x1 + (((4 * t + vc) ^ value_swz<LD>(r1)) << 3))));
+                    const T* const x0 = V + vat[t] + 16 * kk * LD;
+                    const uint2 lo2 =
+                        __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x0));
+                    const uint2 hi2 =
+                        __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(x0 + 8 * LD)));
                     const uint4 vf = make_uint4(lo2.x, lo2.y, hi2.x, hi2.y);
 #pragma unroll
                     for (int b = 0; b < QB; ++b) o[b][t] = mma32<T>(vf, p[b], o[b][t]);
                 }
             }
         }
-        }
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) have[u] = have_next[u];
-        if (st + 1 < steps) {
-            store(st + 1);
-            // the offsets of tile st + 2 replace those of tile st
-            if (asks) locate(st + 2);
-        }
+        if (more) store(st + 1, have_next == ~0ull, next);
+        // the offsets of tile st + kOffs replace those of tile st
+        if (asks) locate(st + kOffs);
+        have = have_next;
         lds_publish_barrier();
+    };
+    if constexpr (DEPTH == 1) {
+        for (int st = 0; st < steps; ++st) step(st, buf[0], buf[0]);
+    } else {
+        for (int st = 0; st < steps; st += 2) {
+            step(st, buf[0], buf[DEPTH - 1]);
+            if (st + 1 < steps) step(st + 1, buf[DEPTH - 1], buf[0]);
+        }
     }
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
@@ -898,7 +934,7 @@ PagedPlan plan(const PagedCall& c) {
         p.blocks = c.dim_qk <= 64 && tall >= kTarget ? 2 : 1;
         p.M = 128 * p.blocks;
         p.KT = kChunkKeys;
-        p.least = 16;
+        p.least = 32;
     } else if (p.kind == kFew) {
         p.blocks = rows <= 16 ? 1 : rows <= 32 || c.dim_qk > 64 ? 2 : 4;
         p.M = kFewRows * p.blocks;
@@ -952,7 +988,7 @@ hipError_t launch_mfma(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
             if (p.blocks == 2)
                 NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 2, 1>), grid, block, lds, s, a);
             else
-                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 2>), grid, block, 2 * lds, s, a);
+                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 2>), grid, block, lds, s, a);
         } else {
             NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 1>), grid, block, lds, s, a);
         }
