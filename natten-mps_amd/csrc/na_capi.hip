@@ -872,10 +872,11 @@ int natten_hip_neighborhood_map(const natten_problem_t* p, int64_t* flat, uint8_
 namespace {
 
 // Elements of a 16-byte (8-byte for some 16-bit heads) vector that divides an
-// axis's pairs and the copied dims, with every operand aligned for it; else 1.
-int rotary_vec(int dtype, int dim, int turned, int axes, int dim_v, std::initializer_list<Run> ts) {
+// axis's pairs (the turned dims, where neighbours pair up) and the copied
+// dims, with every operand aligned for it; else 1.
+int rotary_vec(int dtype, int dim, int turned, int axes, bool interleaved, int dim_v, std::initializer_list<Run> ts) {
     for (int vec : {16 / elem_size(dtype), 4}) {
-        if (turned % (2 * axes * vec) || (dim - turned) % vec || dim_v % vec) continue;
+        if (turned % (interleaved ? vec : 2 * axes * vec) || (dim - turned) % vec || dim_v % vec) continue;
         bool ok = true;
         for (auto& t : ts) {
             if (!t.ptr) continue;
@@ -1013,7 +1014,7 @@ int natten_hip_rotary(const natten_rotary_t* r, const uint64_t* turns, const voi
     c.interleaved = r->interleaved ? 1 : 0;
     c.inverse = r->inverse ? 1 : 0;
     c.magnitude = r->magnitude;
-    c.vec = rotary_vec(r->dtype, r->dim, r->turned, r->axes, 0,
+    c.vec = rotary_vec(r->dtype, r->dim, r->turned, r->axes, r->interleaved != 0, 0,
                        {{r->heads_q ? q : nullptr, lq, r->dim}, {r->heads_q ? q_out : nullptr, lqo, r->dim},
                         {r->heads_k ? k : nullptr, lk, r->dim}, {r->heads_k ? k_out : nullptr, lko, r->dim}});
     return launch_status(na::rotary(c, static_cast<hipStream_t>(stream)), "rotary");
@@ -1057,7 +1058,7 @@ int natten_hip_paged_append(const natten_paged_t* p, const natten_rotary_t* r, c
     c.heads_k = p->heads_kv;
     c.dim = p->dim_qk;
     c.dtype = p->dtype;
-    c.vec = rotary_vec(p->dtype, p->dim_qk, c.turned, 1, p->dim_v,
+    c.vec = rotary_vec(p->dtype, p->dim_qk, c.turned, 1, c.interleaved != 0, p->dim_v,
                        {{q, lq, p->dim_qk}, {q ? q_out : nullptr, lqo, p->dim_qk}, {k, lk, p->dim_qk},
                         {v, lv, p->dim_v}, {key_pages, &lkp, p->dim_qk}, {value_pages, &lvp, p->dim_v}});
     return launch_status(na::paged_append(to_cache(p, key_pages, value_pages, table, seq_lens, new_lens), c, v,

@@ -29,7 +29,7 @@ namespace na {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;           // units of a thread in flight
+constexpr int kUnits = 4;           // units of two vectors of a thread in flight
 constexpr int kMaxTokens = 64;      // tokens per block
 constexpr int kMaxPairs = 128;      // turned pairs of a head (head dim 256)
 constexpr int kAngleFloats = 8192;  // LDS of cosines and sines per block
@@ -89,8 +89,30 @@ __device__ __forceinline__ uint32_t turn_fraction(uint64_t f, int64_t p) {
     return static_cast<uint32_t>((f * static_cast<uint64_t>(p)) >> 32);
 }
 
+// VEC elements as they are moved, in registers of their own.
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<16> {
+    typedef uint32_t type __attribute__((ext_vector_type(4)));
+};
+template <>
+struct Raw<8> {
+    typedef uint32_t type __attribute__((ext_vector_type(2)));
+};
+template <>
+struct Raw<4> {
+    using type = uint32_t;
+};
+template <>
+struct Raw<2> {
+    using type = uint16_t;
+};
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Vec {
+using raw_t = typename Raw<sizeof(T) * VEC>::type;
+
+template <typename T, int VEC>
+struct Vec {
     T x[VEC];
 };
 
@@ -99,28 +121,38 @@ typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
 typedef float f32x2v __attribute__((ext_vector_type(2)));
 
 template <typename T, int VEC>
-__device__ __forceinline__ Vec<T, VEC> round_vec(const float (&f)[VEC]) {
-    Vec<T, VEC> r;
-    if constexpr (std::is_same<T, float>::value || VEC == 1) {
+__device__ __forceinline__ void spread(raw_t<T, VEC> r, float* f) {
+    const Vec<T, VEC> v = __builtin_bit_cast(Vec<T , VEC>, r);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) r.x[i] = from_f<T>(f[i]);
-    } else {
-        using P = typename std::conditional<std::is_same<T, bf16>::value, bf16x2v, f16x2v>::type;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&r);
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i)
-            w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2v{f[2 * i], f[2 * i + 1]}), P));
-    }
-    return r;
+    for (int i = 0; i < VEC; ++i) f[i] = to_f(v.x[i]);
 }
 
-// One unit of work: VEC pairs of a head (two vectors), or one vector that is
-// copied (dims that do not turn, and values).
 template <typename T, int VEC>
+__device__ __forceinline__ raw_t<T, VEC> round_vec(const float* f) {
+    if constexpr (std::is_same<T, float>::value || VEC == 1) {
+        Vec<T, VEC> r;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) r.x[i] = from_f<T>(f[i]);
+        return __builtin_bit_cast(raw_t<T , VEC>, r);
+    } else {
+        using P = typename std::conditional<std::is_same<T, bf16>::value, bf16x2v, f16x2v>::type;
+        struct Pairs {
+            P p[VEC / 2];
+        } r;
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) r.p[i] = __builtin_convertvector((f32x2v{f[2 * i], f[2 * i + 1]}), P);
+        return __builtin_bit_cast(raw_t<T , VEC>, r);
+    }
+}
+
+// One unit of work: two vectors of a head that hold VEC pairs, `gap` elements
+// apart (neighbours that pair up: one vector of VEC / 2 pairs, gap 0), or one
+// vector that is copied (angle -1: dims that do not turn, and values).
+template <typename T>
 struct Unit {
     const T* src;
     T* dst;
-    int gap;    // elements from the first vector to the second; 0: a copy
+    int gap;
     int angle;  // first pair's index among the block's angles
     int zero;   // padding: zeros are written
 };
@@ -171,7 +203,75 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
             coord[t][2] = i2;
         }
     }
-    if (PAGED || !a.pos_bits) __syncthreads();
+    __syncthreads();
+
+    // The block's first loads go out before its angles are computed.
+    using R = raw_t<T, VEC>;
+    constexpr bool kOne = INTER && VEC > 1;
+    constexpr int kBatch = kOne ? 2 * kUnits : kUnits;
+    const int turning = kOne ? a.turned / VEC : a.half / VEC;  // units of a head that turn
+    const int uqk = (a.hq + a.hk) * static_cast<int>(a.fhead.d);
+    const int total = nt * static_cast<int>(a.funits.d);
+    Unit<T> u[kBatch];
+    R x[kBatch], y[kBatch];
+    auto fetch = [&](int e0) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int e = e0 + i * kThreads;
+            u[i].dst = nullptr;
+            if (e >= total) continue;
+            const int t = fdiv(e, a.funits);
+            int r = e - t * static_cast<int>(a.funits.d);
+            u[i].zero = 0;
+            u[i].gap = 0;
+            u[i].angle = -1;
+            if (r < uqk) {
+                int h = fdiv(r, a.fhead);
+                const int w = r - h * static_cast<int>(a.fhead.d);
+                const bool isq = h < a.hq;
+                if (!isq) h -= a.hq;
+                const long long so = isq ? off[t][0] : off[t][2], to = isq ? off[t][1] : off[t][3];
+                if (PAGED && !isq && to < 0) continue;
+                int d;
+                if (w < turning) {
+                    if constexpr (kOne) {
+                        u[i].angle = t * a.half + w * (VEC / 2);
+                        d = w * VEC;
+                    } else if constexpr (INTER) {
+                        u[i].angle = t * a.half + w;
+                        u[i].gap = 1;
+                        d = 2 * w;
+                    } else {
+                        u[i].angle = t * a.half + w * VEC;
+                        int ax = 0, j = w * VEC;
+                        while (ax + 1 < a.axes && j >= a.pairs) {
+                            j -= a.pairs;
+                            ++ax;
+                        }
+                        d = 2 * ax * a.pairs + j;
+                        u[i].gap = a.pairs;
+                    }
+                } else {
+                    d = a.turned + (w - turning) * VEC;
+                }
+                u[i].zero = PAGED && isq && so < 0;
+                u[i].src = static_cast<const T*>(isq ? a.q : a.k) + (so + h * (isq ? a.lq.h : a.lk.h) + d);
+                u[i].dst = static_cast<T*>(isq ? a.qo : a.ko) + (to + h * (isq ? a.lqo.h : a.lko.h) + d);
+            } else if (PAGED) {
+                r -= uqk;
+                const int h = fdiv(r, a.fvhead), w = r - h * static_cast<int>(a.fvhead.d);
+                const long long to = off[t][5];
+                if (to < 0) continue;
+                u[i].src = static_cast<const T*>(a.v) + (off[t][4] + h * a.lv.h + w * VEC);
+                u[i].dst = static_cast<T*>(a.vo) + (to + h * a.lvo.h + w * VEC);
+            }
+            if (!u[i].zero) {
+                x[i] = *reinterpret_cast<const R*>(u[i].src);
+                if (u[i].gap) y[i] = *reinterpret_cast<const R*>(u[i].src + u[i].gap);
+            }
+        }
+    };
+    fetch(tid);
 
     const int nangle = nt * a.half;
     float* const cosv = angles;
@@ -198,98 +298,44 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
         sinv[e] = r.s * (a.mag * a.dir);
     }
     lds_publish_barrier();
-
-    const int turning = a.half / VEC;  // units of a head that turn
-    const int uqk = (a.hq + a.hk) * static_cast<int>(a.fhead.d);
-    const int total = nt * static_cast<int>(a.funits.d);
     for (int e0 = tid; e0 < total; e0 += kThreads * kBatch) {
-        Unit<T, VEC> u[kBatch];
-        Vec<T, VEC> x[kBatch], y[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int e = e0 + i * kThreads;
-            u[i].dst = nullptr;
-            if (e >= total) continue;
-            const int t = fdiv(e, a.funits);
-            int r = e - t * static_cast<int>(a.funits.d);
-            u[i].zero = 0;
-            u[i].gap = 0;
-            u[i].angle = 0;
-            if (r < uqk) {
-                int h = fdiv(r, a.fhead);
-                const int w = r - h * static_cast<int>(a.fhead.d);
-                const bool isq = h < a.hq;
-                if (!isq) h -= a.hq;
-                const long long so = isq ? off[t][0] : off[t][2], to = isq ? off[t][1] : off[t][3];
-                if (PAGED && !isq && to < 0) continue;
-                int d;
-                if (w < turning) {
-                    u[i].angle = t * a.half + w * VEC;
-                    if constexpr (INTER) {
-                        d = 2 * w * VEC;
-                        u[i].gap = VEC;
-                    } else {
-                        int ax = 0, j = w * VEC;
-                        while (ax + 1 < a.axes && j >= a.pairs) {
-                            j -= a.pairs;
-                            ++ax;
-                        }
-                        d = 2 * ax * a.pairs + j;
-                        u[i].gap = a.pairs;
-                    }
-                } else {
-                    d = a.turned + (w - turning) * VEC;
-                }
-                u[i].zero = PAGED && isq && so < 0;
-                u[i].src = static_cast<const T*>(isq ? a.q : a.k) + (so + h * (isq ? a.lq.h : a.lk.h) + d);
-                u[i].dst = static_cast<T*>(isq ? a.qo : a.ko) + (to + h * (isq ? a.lqo.h : a.lko.h) + d);
-            } else if (PAGED) {
-                r -= uqk;
-                const int h = fdiv(r, a.fvhead), w = r - h * static_cast<int>(a.fvhead.d);
-                const long long to = off[t][5];
-                if (to < 0) continue;
-                u[i].src = static_cast<const T*>(a.v) + (off[t][4] + h * a.lv.h + w * VEC);
-                u[i].dst = static_cast<T*>(a.vo) + (to + h * a.lvo.h + w * VEC);
-            }
-            if (!u[i].zero) {
-                x[i] = *reinterpret_cast<const Vec<T, VEC>*>(u[i].src);
-                if (u[i].gap) y[i] = *reinterpret_cast<const Vec<T, VEC>*>(u[i].src + u[i].gap);
-            }
-        }
+        if (e0 != tid) fetch(e0);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             if (!u[i].dst) continue;
+            R* const to = reinterpret_cast<R*>(u[i].dst);
+            R* const to2 = reinterpret_cast<R*>(u[i].dst + u[i].gap);
             if (u[i].zero) {
-                Vec<T, VEC> z{};
-                *reinterpret_cast<Vec<T, VEC>*>(u[i].dst) = z;
-                if (u[i].gap) *reinterpret_cast<Vec<T, VEC>*>(u[i].dst + u[i].gap) = z;
+                *to = R{};
+                if (u[i].gap) *to2 = R{};
                 continue;
             }
-            if (u[i].gap) {
-                float p[2 * VEC];
-                float lo[VEC], hi[VEC];
+            if (u[i].angle < 0) {
+                *to = x[i];
+                continue;
+            }
+            if constexpr (kOne) {
+                float p[VEC], o[VEC];
+                spread<T, VEC>(x[i], p);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    p[j] = to_f(x[i].x[j]);
-                    p[VEC + j] = to_f(y[i].x[j]);
+                for (int j = 0; j < VEC / 2; ++j) {
+                    const float c = cosv[u[i].angle + j], s = sinv[u[i].angle + j];
+                    o[2 * j] = fmaf(p[2 * j], c, -(p[2 * j + 1] * s));
+                    o[2 * j + 1] = fmaf(p[2 * j], s, p[2 * j + 1] * c);
                 }
-                float o[2 * VEC];
+                *to = round_vec<T, VEC>(o);
+            } else {
+                float p[VEC], q[VEC], o1[VEC], o2[VEC];
+                spread<T, VEC>(x[i], p);
+                spread<T, VEC>(y[i], q);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     const float c = cosv[u[i].angle + j], s = sinv[u[i].angle + j];
-                    const float pu = INTER ? p[2 * j] : p[j], pv = INTER ? p[2 * j + 1] : p[VEC + j];
-                    o[INTER ? 2 * j : j] = fmaf(pu, c, -(pv * s));
-                    o[INTER ? 2 * j + 1 : VEC + j] = fmaf(pu, s, pv * c);
+                    o1[j] = fmaf(p[j], c, -(q[j] * s));
+                    o2[j] = fmaf(p[j], s, q[j] * c);
                 }
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    lo[j] = o[j];
-                    hi[j] = o[VEC + j];
-                }
-                *reinterpret_cast<Vec<T, VEC>*>(u[i].dst) = round_vec<T, VEC>(lo);
-                *reinterpret_cast<Vec<T, VEC>*>(u[i].dst + u[i].gap) = round_vec<T, VEC>(hi);
-            } else {
-                *reinterpret_cast<Vec<T, VEC>*>(u[i].dst) = x[i];
+                *to = round_vec<T, VEC>(o1);
+                *to2 = round_vec<T, VEC>(o2);
             }
         }
     }
@@ -311,16 +357,19 @@ template <bool PAGED>
 hipError_t launch_any(RotaryArgs& a, int dtype, int vec, bool inter, int dim_v, hipStream_t s) {
     a.half = a.turned / 2;
     a.pairs = a.half / a.axes;
-    const int uh = a.half / vec + (a.dim - a.turned) / vec, uv = PAGED ? dim_v / vec : 0;
+    // units of a head: see k_rotary
+    const int turning = inter && vec > 1 ? a.turned / vec : a.half / vec;
+    const int uh = turning + (a.dim - a.turned) / vec, uv = PAGED ? dim_v / vec : 0;
     const int units = (a.hq + a.hk) * uh + a.hv * uv;
     a.fpairs = make_fastdiv(imax(a.half, 1));
     a.fhead = make_fastdiv(imax(uh, 1));
     a.fvhead = make_fastdiv(imax(uv, 1));
     a.funits = make_fastdiv(units);
-    // Tokens per block: up to kBatch units a thread, as long as that leaves
+    // Tokens per block: up to a batch of units a thread, as long as that leaves
     // four blocks a compute unit; the angles of a block fit their LDS.
     int tb = 1;
-    while (tb < kMaxTokens && 2 * tb * units <= kThreads * kBatch && 2 * tb * 1024 <= a.tokens) tb *= 2;
+    const int batch = inter && vec > 1 ? 2 * kUnits : kUnits;
+    while (tb < kMaxTokens && 2 * tb * units <= kThreads * batch && 2 * tb * 1024 <= a.tokens) tb *= 2;
     while (tb > 1 && 2 * tb * a.half > kAngleFloats) tb /= 2;
     a.tb = tb;
     if (dtype == NATTEN_F32) {
