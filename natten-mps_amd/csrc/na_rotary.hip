@@ -29,7 +29,7 @@ namespace na {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnits = 4;           // units of two vectors of a thread in flight
+constexpr int kUnits = 4;           // units of a thread in flight
 constexpr int kMaxTokens = 64;      // tokens per block
 constexpr int kMaxPairs = 128;      // turned pairs of a head (head dim 256)
 constexpr int kAngleFloats = 8192;  // LDS of cosines and sines per block
@@ -145,6 +145,14 @@ __device__ __forceinline__ raw_t<T, VEC> round_vec(const float* f) {
     }
 }
 
+template <bool STREAM, typename R>
+__device__ __forceinline__ void put(R* to, R v) {
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(v, to);
+    else
+        *to = v;
+}
+
 // One unit of work: two vectors of a head that hold VEC pairs, `gap` elements
 // apart (neighbours that pair up: one vector of VEC / 2 pairs, gap 0), or one
 // vector that is copied (angle -1: dims that do not turn, and values).
@@ -157,7 +165,8 @@ struct Unit {
     int zero;   // padding: zeros are written
 };
 
-template <typename T, int VEC, bool INTER, bool PAGED>
+// STREAM: results go past the caches.
+template <typename T, int VEC, bool INTER, bool PAGED, bool STREAM>
 __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
     extern __shared__ float angles[];  // [tb * half] cosines, then sines
     __shared__ long long off[kMaxTokens][6];
@@ -208,15 +217,14 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
     // The block's first loads go out before its angles are computed.
     using R = raw_t<T, VEC>;
     constexpr bool kOne = INTER && VEC > 1;
-    constexpr int kBatch = kOne ? 2 * kUnits : kUnits;
     const int turning = kOne ? a.turned / VEC : a.half / VEC;  // units of a head that turn
     const int uqk = (a.hq + a.hk) * static_cast<int>(a.fhead.d);
     const int total = nt * static_cast<int>(a.funits.d);
-    Unit<T> u[kBatch];
-    R x[kBatch], y[kBatch];
+    Unit<T> u[kUnits];
+    R x[kUnits], y[kUnits];
     auto fetch = [&](int e0) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < kUnits; ++i) {
             const int e = e0 + i * kThreads;
             u[i].dst = nullptr;
             if (e >= total) continue;
@@ -298,10 +306,10 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
         sinv[e] = r.s * (a.mag * a.dir);
     }
     lds_publish_barrier();
-    for (int e0 = tid; e0 < total; e0 += kThreads * kBatch) {
+    for (int e0 = tid; e0 < total; e0 += kThreads * kUnits) {
         if (e0 != tid) fetch(e0);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < kUnits; ++i) {
             if (!u[i].dst) continue;
             R* const to = reinterpret_cast<R*>(u[i].dst);
             R* const to2 = reinterpret_cast<R*>(u[i].dst + u[i].gap);
@@ -311,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
                 continue;
             }
             if (u[i].angle < 0) {
-                *to = x[i];
+                put<STREAM>(to, x[i]);
                 continue;
             }
             if constexpr (kOne) {
@@ -323,7 +331,7 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
                     o[2 * j] = fmaf(p[2 * j], c, -(p[2 * j + 1] * s));
                     o[2 * j + 1] = fmaf(p[2 * j], s, p[2 * j + 1] * c);
                 }
-                *to = round_vec<T, VEC>(o);
+                put<STREAM>(to, round_vec<T, VEC>(o));
             } else {
                 float p[VEC], q[VEC], o1[VEC], o2[VEC];
                 spread<T, VEC>(x[i], p);
@@ -334,22 +342,31 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
                     o1[j] = fmaf(p[j], c, -(q[j] * s));
                     o2[j] = fmaf(p[j], s, q[j] * c);
                 }
-                *to = round_vec<T, VEC>(o1);
-                *to2 = round_vec<T, VEC>(o2);
+                put<STREAM>(to, round_vec<T, VEC>(o1));
+                put<STREAM>(to2, round_vec<T, VEC>(o2));
             }
         }
     }
 }
 
 template <typename T, int VEC, bool PAGED>
-hipError_t launch(const RotaryArgs& a, bool inter, hipStream_t s) {
-    const int blocks = (a.tokens + a.tb - 1) / a.tb;
+hipError_t launch(const RotaryArgs& a, bool inter, bool stream, hipStream_t s) {
+    const dim3 grid((a.tokens + a.tb - 1) / a.tb), block(kThreads);
     const size_t shm = sizeof(float) * 2 * static_cast<size_t>(a.tb) * a.half;
     const char* const name = PAGED ? "na_paged_append" : "na_rotary";
+    if constexpr (VEC > 1) {
+        if (stream) {
+            if (inter)
+                NA_LAUNCH(name, (k_rotary<T, VEC, true, PAGED, true>), grid, block, shm, s, a);
+            else
+                NA_LAUNCH(name, (k_rotary<T, VEC, false, PAGED, true>), grid, block, shm, s, a);
+            return hipGetLastError();
+        }
+    }
     if (inter)
-        NA_LAUNCH(name, (k_rotary<T, VEC, true, PAGED>), dim3(blocks), dim3(kThreads), shm, s, a);
+        NA_LAUNCH(name, (k_rotary<T, VEC, true, PAGED, false>), grid, block, shm, s, a);
     else
-        NA_LAUNCH(name, (k_rotary<T, VEC, false, PAGED>), dim3(blocks), dim3(kThreads), shm, s, a);
+        NA_LAUNCH(name, (k_rotary<T, VEC, false, PAGED, false>), grid, block, shm, s, a);
     return hipGetLastError();
 }
 
@@ -361,6 +378,7 @@ hipError_t launch_any(RotaryArgs& a, int dtype, int vec, bool inter, int dim_v, 
     const int turning = inter && vec > 1 ? a.turned / vec : a.half / vec;
     const int uh = turning + (a.dim - a.turned) / vec, uv = PAGED ? dim_v / vec : 0;
     const int units = (a.hq + a.hk) * uh + a.hv * uv;
+    const int elem = dtype == NATTEN_F32 ? 4 : 2;
     a.fpairs = make_fastdiv(imax(a.half, 1));
     a.fhead = make_fastdiv(imax(uh, 1));
     a.fvhead = make_fastdiv(imax(uv, 1));
@@ -368,22 +386,28 @@ hipError_t launch_any(RotaryArgs& a, int dtype, int vec, bool inter, int dim_v, 
     // Tokens per block: up to a batch of units a thread, as long as that leaves
     // four blocks a compute unit; the angles of a block fit their LDS.
     int tb = 1;
-    const int batch = inter && vec > 1 ? 2 * kUnits : kUnits;
-    while (tb < kMaxTokens && 2 * tb * units <= kThreads * batch && 2 * tb * 1024 <= a.tokens) tb *= 2;
+    while (tb < kMaxTokens && 2 * tb * units <= kThreads * kUnits && 2 * tb * 1024 <= a.tokens) tb *= 2;
     while (tb > 1 && 2 * tb * a.half > kAngleFloats) tb /= 2;
     a.tb = tb;
+    // Results that no cache can hold for their reader are stored past them,
+    // if a store instruction writes runs of 64 bytes: 168 MB at heads of 64
+    // (runs of 64) 36 -> 31 us, 205 MB interleaved 44 -> 34 us; at runs of 16
+    // bytes (three axes of 16 dims) it would be 31 -> 67 us.
+    const long long bytes = elem * a.tokens * (static_cast<long long>(a.hq + a.hk) * a.dim + static_cast<long long>(a.hv) * dim_v);
+    const int rest = a.dim - a.turned;
+    const bool stream = bytes >= (32ll << 20) && (inter || a.pairs * elem >= 64) && (!rest || rest * elem >= 64);
     if (dtype == NATTEN_F32) {
-        if (vec == 4) return launch<float, 4, PAGED>(a, inter, s);
-        return launch<float, 1, PAGED>(a, inter, s);
+        if (vec == 4) return launch<float, 4, PAGED>(a, inter, stream, s);
+        return launch<float, 1, PAGED>(a, inter, stream, s);
     }
     if (dtype == NATTEN_F16) {
-        if (vec == 8) return launch<f16, 8, PAGED>(a, inter, s);
-        if (vec == 4) return launch<f16, 4, PAGED>(a, inter, s);
-        return launch<f16, 1, PAGED>(a, inter, s);
+        if (vec == 8) return launch<f16, 8, PAGED>(a, inter, stream, s);
+        if (vec == 4) return launch<f16, 4, PAGED>(a, inter, stream, s);
+        return launch<f16, 1, PAGED>(a, inter, stream, s);
     }
-    if (vec == 8) return launch<bf16, 8, PAGED>(a, inter, s);
-    if (vec == 4) return launch<bf16, 4, PAGED>(a, inter, s);
-    return launch<bf16, 1, PAGED>(a, inter, s);
+    if (vec == 8) return launch<bf16, 8, PAGED>(a, inter, stream, s);
+    if (vec == 4) return launch<bf16, 4, PAGED>(a, inter, stream, s);
+    return launch<bf16, 1, PAGED>(a, inter, stream, s);
 }
 
 }  // namespace
