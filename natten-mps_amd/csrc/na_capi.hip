@@ -911,8 +911,12 @@ int check_paged(const natten_paged_t* p) {
     if (p->table_stride < 0) return fail(NATTEN_ERR_INVALID, "negative table stride");
     for (int i = 0; i < 3; ++i)
         if (p->key_stride[i] < 0 || p->value_stride[i] < 0) return fail(NATTEN_ERR_INVALID, "negative page stride");
-    if (static_cast<long long>(p->batch) * p->tokens * (p->heads_q > 0 ? p->heads_q : 1) > (1ll << 30))
-        return fail(NATTEN_ERR_UNSUPPORTED, "batch x tokens x heads above 2^30");
+    // rows, waves and key positions are counted in 32 bits
+    if (static_cast<long long>(p->batch) * p->tokens > (1ll << 27) ||
+        static_cast<long long>(p->batch) * p->tokens * (p->heads_q > 0 ? p->heads_q : 1) > (1ll << 27))
+        return fail(NATTEN_ERR_UNSUPPORTED, "batch x tokens x heads above 2^27");
+    if (static_cast<long long>(p->table_width) * p->page_size > 0x7fffffffll - 4096)
+        return fail(NATTEN_ERR_UNSUPPORTED, "a table of more than 2^31 - 4097 positions");
     return NATTEN_OK;
 }
 

@@ -8,11 +8,12 @@
 // the scale carries log2 e).
 //
 // k_paged_rows  any type, head dims to 256, any alignment: a wave per row.
-// k_paged_few   16-bit, head dim 32/64/96/128: 16 rows a workgroup on MFMA,
-//               its four waves on different keys.  The cache is read once, so
-//               HBM bounds it.
-// k_paged_chunk the same types, many rows: 128 or 256 rows a workgroup on
-//               MFMA, keys and values staged in LDS for all its waves.
+// k_paged_few   head dims 32/64/96/128, aligned: 16 to 64 rows a workgroup on
+//               MFMA, its four waves on different keys.  With few rows the
+//               cache is read once and HBM bounds it.  fp32 takes it for any
+//               number of rows.
+// k_paged_chunk 16-bit, many rows: 128 or 256 rows a workgroup on MFMA, keys
+//               and values staged in LDS for all its waves.
 // k_paged_join  joins the parts of tiles whose keys were cut.
 #include <type_traits>
 
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_rows(PagedArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// 16-bit types on MFMA
+// on MFMA
 // ---------------------------------------------------------------------------
 
 // Elements of an LDS row of head dim D, and the swizzle of its 16-byte pieces:
@@ -177,13 +178,14 @@ constexpr float kSlack = 8.f;
 // zero, so that scores times `sc2` > 0 order as the logits do.
 struct ScaleParts {
     float sc2;
-    uint32_t flip, keep;  // of two 16-bit elements
+    uint32_t flip, keep;  // of a word: one element, or two 16-bit ones
 };
 
+template <typename T>
 __device__ __forceinline__ ScaleParts scale_parts(float scale) {
     ScaleParts r;
     r.sc2 = scale == 0.f ? 1.f : __builtin_fabsf(scale) * kLog2e;
-    r.flip = scale < 0.f ? 0x80008000u : 0u;
+    r.flip = scale < 0.f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;
     r.keep = scale == 0.f ? 0u : 0xffffffffu;
     return r;
 }
@@ -236,11 +238,38 @@ __device__ __forceinline__ bool four_nonfinite(f32x4_t x) { return item_nonfinit
 // Each key is read once per kv head and nothing else is big, so HBM bounds
 // it: the next keys' loads are issued as soon as the registers are free, and
 // page numbers one step before that.
-constexpr int kFewRows = 16, kFewKeys = 32;
+//
+// fp32 takes v_mfma 16x16x4, 16 keys at a time: element e of the 16-byte
+// pieces is one product's k slot (both operands permuted alike), and a lane's
+// four keys of a block are the k slots of four products with V, whose operand
+// needs no transposition.
+constexpr int kFewRows = 16;
+template <typename T>
+constexpr int few_keys() {
+    return sizeof(T) == 4 ? 16 : 32;
+}
+
+typedef float f32x4v_t __attribute__((ext_vector_type(4)));
+
+// Swizzle of a row's 16-byte pieces in k_paged_few's LDS.
+template <typename T, int D>
+__device__ __forceinline__ int few_swz(int row) {
+    if constexpr (sizeof(T) == 4) return row & (D == 32 ? 7 : 15);
+    else return piece_swz<D>(row);
+}
+
+// Waves a SIMD that leave the kernel its registers.
+template <typename T>
+constexpr int few_waves(int dim, int blocks) {
+    if (sizeof(T) == 4) return blocks == 1 ? (dim > 64 ? 2 : 4) : dim > 96 ? 1 : 2;
+    return blocks > 1 || dim > 96 ? 2 : dim > 64 ? 3 : 4;
+}
 
 template <typename T, int D, int NB>
-__global__ __launch_bounds__(kPagedThreads, NB > 1 ? 2 : D > 64 ? 3 : 4) void k_paged_few(PagedArgs a) {
-    constexpr int C = D / 32, LD = row_elems<D>(), DB = D / 16;
+__global__ __launch_bounds__(kPagedThreads, few_waves<T>(D, NB)) void k_paged_few(PagedArgs a) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int E = 16 / sizeof(T), C = D / (4 * E);  // elements of a piece, pieces of a lane in a row
+    constexpr int LD = row_elems<D>(), DB = D / 16, KS = few_keys<T>(), KB = KS / 16;
     constexpr int kRowsOf = kFewRows * NB;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ float ml[4][kRowsOf][2];
@@ -250,7 +279,7 @@ __global__ __launch_bounds__(kPagedThreads, NB > 1 ? 2 : D > 64 ? 3 : 4) void k_
     if (r.rows <= 0) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int col = lane & 15, g = lane >> 4;
-    const ScaleParts sp = scale_parts(a.scale);
+    const ScaleParts sp = scale_parts<T>(a.scale);
     // queries, their windows, and what all rows of the tile see
     uint4 qf[NB][C];
     int hi[NB];
@@ -264,42 +293,42 @@ __global__ __launch_bounds__(kPagedThreads, NB > 1 ? 2 : D > 64 ? 3 : 4) void k_
     for (int n = 0; n < NB; ++n) {
         const T* const q = query(n);
 #pragma unroll
-        for (int c = 0; c < C; ++c) qf[n][c] = scaled(*reinterpret_cast<const uint4*>(q + 32 * c + 8 * g), sp);
+        for (int c = 0; c < C; ++c) qf[n][c] = scaled(*reinterpret_cast<const uint4*>(q + E * (4 * c + g)), sp);
         hi[n] = r.w0 + fdiv(r.row0 + imin(16 * n + col, r.rows - 1), a.frep);
     }
     const int all_hi = imin(r.w0 + fdiv(r.row0, a.frep), r.u_hi);
     const int all_lo = a.K ? r.w0 + fdiv(r.row0 + r.rows - 1, a.frep) - a.K + 1 : 0;
-    const int steps = (r.u_hi - r.u_lo + kFewKeys) / kFewKeys;  // 0 when empty: u_hi = u_lo - 1 at least
+    const int steps = (r.u_hi - r.u_lo + KS) / KS;  // 0 when empty: u_hi = u_lo - 1 at least
     const int* const table = a.table + r.b * a.table_stride;
-    const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh + 8 * g;
-    const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh + 8 * g;
-    T* const X = reinterpret_cast<T*>(lds) + wave * (kFewKeys * LD);
+    const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh + E * g;
+    const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh + E * g;
+    T* const X = reinterpret_cast<T*>(lds) + wave * (KS * LD);
 
-    int page[2], slot[2];
+    int page[KB], slot[KB];
     auto lookup = [&](int st) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int u = imin(r.u_lo + st * kFewKeys + 16 * b + col, r.u_hi);
+        for (int b = 0; b < KB; ++b) {
+            const int u = imin(r.u_lo + st * KS + 16 * b + col, r.u_hi);
             const int j = r.c + u * a.dil;
             const int pg = fdiv(j, a.fpage);
             slot[b] = j - pg * a.page_size;
             page[b] = table[pg];
         }
     };
-    uint4 kf[2][C], vf[2][C];
-    bool ok[2];
+    uint4 kf[KB][C], vf[KB][C];
+    bool ok[KB];
     auto load = [&](int st) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            ok[b] = page[b] >= 0 && page[b] < a.pages && r.u_lo + st * kFewKeys + 16 * b + col <= r.u_hi;
+        for (int b = 0; b < KB; ++b) {
+            ok[b] = page[b] >= 0 && page[b] < a.pages && r.u_lo + st * KS + 16 * b + col <= r.u_hi;
             // keys that are not there: the pool's first slot, masked below
             const int pg = ok[b] ? page[b] : 0, sl = ok[b] ? slot[b] : 0;
             const T* const k = kb + (pg * a.kp + sl * a.ks);
             const T* const v = vb + (pg * a.vp + sl * a.vs);
 #pragma unroll
-            for (int c = 0; c < C; ++c) kf[b][c] = *reinterpret_cast<const uint4*>(k + 32 * c);
+            for (int c = 0; c < C; ++c) kf[b][c] = *reinterpret_cast<const uint4*>(k + 4 * E * c);
 #pragma unroll
-            for (int c = 0; c < C; ++c) vf[b][c] = *reinterpret_cast<const uint4*>(v + 32 * c);
+            for (int c = 0; c < C; ++c) vf[b][c] = *reinterpret_cast<const uint4*>(v + 4 * E * c);
         }
     };
 
@@ -318,50 +347,70 @@ __global__ __launch_bounds__(kPagedThreads, NB > 1 ? 2 : D > 64 ? 3 : 4) void k_
         if (wave + 4 < steps) lookup(wave + 4);
     }
     for (int st = wave; st < steps; st += 4) {
-        const int ub = r.u_lo + st * kFewKeys;
-        f32x4_t s[NB][2];
+        const int ub = r.u_lo + st * KS;
+        f32x4_t s[NB][KB];
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < KB; ++b) {
                 s[n][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < C; ++c) s[n][b] = Mma<T>::run(kf[b][c], qf[n][c], s[n][b]);
-            }
-        const bool there[2] = {ok[0], ok[1]};
-        const unsigned long long have0 = __ballot(there[0]), have1 = __ballot(there[1]);
-        const bool whole = (have0 & have1) == ~0ull;
+                for (int c = 0; c < C; ++c) {
+                    if constexpr (F32) {
+                        const f32x4v_t x = __builtin_bit_cast(f32x4v_t, kf[b][c]);
+                        const f32x4v_t y = __builtin_bit_cast(f32x4v_t, qf[n][c]);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const int rw = 16 * b + col, sw = piece_swz<D>(rw);
+                        for (int e = 0; e < 4; ++e)
+                            s[n][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], s[n][b], 0, 0, 0);
+                    } else {
+                        s[n][b] = Mma<T>::run(kf[b][c], qf[n][c], s[n][b]);
+                    }
+                }
+            }
+        bool there[KB];
+        unsigned long long have[KB];
+        bool whole = true;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            there[b] = ok[b];
+            have[b] = __ballot(there[b]);
+            whole = whole && have[b] == ~0ull;
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int rw = 16 * b + col, sw = few_swz<T, D>(rw);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 uint4 x = vf[b][c];
                 if (!whole && !there[b]) x = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(X + rw * LD + (((4 * c + g) ^ sw) << 3)) = x;
+                *reinterpret_cast<uint4*>(X + rw * LD + ((4 * c + g) ^ sw) * E) = x;
             }
         }
         if (st + 4 < steps) {
             load(st + 4);
             if (st + 8 < steps) lookup(st + 8);
         }
-        if (!whole || ub + kFewKeys - 1 > all_hi || ub < all_lo) {
-            const uint32_t bits[2] = {static_cast<uint32_t>(have0 >> (4 * g)), static_cast<uint32_t>(have1 >> (4 * g))};
+        if (!whole || ub + KS - 1 > all_hi || ub < all_lo) {
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 // keys ahead of the query count as far behind it
                 const uint32_t back = static_cast<uint32_t>(hi[n] - ub - 4 * g);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int b = 0; b < KB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (back - (16 * b + i) > reach || !((bits[b] >> i) & 1)) s[n][b][i] = -INFINITY;
+                        if (back - (16 * b + i) > reach || !((static_cast<uint32_t>(have[b]) >> (4 * g + i)) & 1)) s[n][b][i] = -INFINITY;
             }
         }
-        uint4 p[NB];
+        uint4 p[F32 ? 1 : NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            const float top = max_rows(max8(s[n])) * sp.sc2;
+            float top;
+            if constexpr (KB == 2)
+                top = max8(s[n]);
+            else
+                top = fmaxp(fmaxp(s[n][0][0], s[n][0][1]), fmaxp(s[n][0][2], s[n][0][3]));
+            top = max_rows(top) * sp.sc2;
             const bool raise = top > m[n] + kSlack;
             if (__ballot(raise)) {
                 const float m2 = raise ? top : m[n];
@@ -373,26 +422,40 @@ __global__ __launch_bounds__(kPagedThreads, NB > 1 ? 2 : D > 64 ? 3 : 4) void k_
             }
             const float ref = m[n] == -INFINITY ? 0.f : m[n];
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     s[n][b][i] = __builtin_amdgcn_exp2f(fmaf(s[n][b][i], sp.sc2, -ref));
                     l[n] += s[n][b][i];
                 }
-            p[n] = pack8<T>(s[n]);
+            if constexpr (!F32) p[n] = pack8<T>(s[n]);
         }
-        const int r0 = 4 * g + (col >> 2), r1 = 16 + r0;
-        const int s0 = piece_swz<D>(r0), s1 = piece_swz<D>(r1);
+        if constexpr (F32) {
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-            const int pc = 2 * db + ((col & 3) >> 1);
-            const T* const x0 = X + r0 * LD + ((pc ^ s0) << 3) + (col & 1) * 4;
-            const T* const x1 = X + r1 * LD + ((pc ^ s1) << 3) + (col & 1) * 4;
-            const uint2 lo2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x0));
-            const uint2 hi2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x1));
-            const uint4 x = make_uint4(lo2.x, lo2.y, hi2.x, hi2.y);
+            for (int i = 0; i < 4; ++i) {
+                const int rw = 4 * g + i;
 #pragma unroll
-            for (int n = 0; n < NB; ++n) o[n][db] = Mma<T>::run(x, p[n], o[n][db]);
+                for (int db = 0; db < DB; ++db) {
+                    const float x = X[rw * LD + ((4 * db + (col >> 2)) ^ few_swz<T, D>(rw)) * 4 + (col & 3)];
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+                        o[n][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, s[n][0][i], o[n][db], 0, 0, 0);
+                }
+            }
+        } else {
+            const int r0 = 4 * g + (col >> 2), r1 = 16 + r0;
+            const int s0 = piece_swz<D>(r0), s1 = piece_swz<D>(r1);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                const int pc = 2 * db + ((col & 3) >> 1);
+                const T* const x0 = X + r0 * LD + ((pc ^ s0) << 3) + (col & 1) * 4;
+                const T* const x1 = X + r1 * LD + ((pc ^ s1) << 3) + (col & 1) * 4;
+                const uint2 lo2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x0));
+                const uint2 hi2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x1));
+                const uint4 x = make_uint4(lo2.x, lo2.y, hi2.x, hi2.y);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[n][db] = Mma<T>::run(x, p[n], o[n][db]);
+            }
         }
     }
     // the four waves' parts, through the LDS that held their values
@@ -437,8 +500,11 @@ __global__ __launch_bounds__(kPagedThreads, NB > 1 ? 2 : D > 64 ? 3 : 4) void k_
         int i, hq;
         row_token(a, r.cls, r.h, r.row0 + rw, i, hq);
         T* const out = static_cast<T*>(a.out) + r.b * a.lo.b + i * a.lo.s2 + hq * a.lo.h + d;
-        *reinterpret_cast<uint2*>(out) = make_uint2(Mma<T>::pack(x[0] * inv, x[1] * inv),
-                                                    Mma<T>::pack(x[2] * inv, x[3] * inv));
+        if constexpr (F32)
+            *reinterpret_cast<f32x4_t*>(out) = x * inv;
+        else
+            *reinterpret_cast<uint2*>(out) = make_uint2(Mma<T>::pack(x[0] * inv, x[1] * inv),
+                                                        Mma<T>::pack(x[2] * inv, x[3] * inv));
         if (d == 0) a.lse[r.b * a.ll.b + i * a.ll.s2 + hq * a.ll.h] = row_lse(mt, lt);
     }
 }
@@ -509,7 +575,7 @@ __global__ __launch_bounds__(kPagedThreads, DEPTH == 2 ? 3 : 2) void k_paged_chu
     if (r.rows <= 0) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int col = lane & 31, h = lane >> 5;
-    const ScaleParts sp = scale_parts(a.scale);
+    const ScaleParts sp = scale_parts<T>(a.scale);
     const int* const table = a.table + r.b * a.table_stride;
     const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh;
     const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh;
@@ -913,11 +979,11 @@ constexpr int exponent_of(int n) { return n <= 1 ? 0 : 1 + exponent_of(n / 2); }
 
 long long padded(long long bytes) { return (bytes + 255) & ~255ll; }
 
-// MFMA kernels: 16-bit, equal head dims that they are built for, operands
-// read and written in 16-byte vectors.
+// MFMA kernels: equal head dims that they are built for, operands read and
+// written in 16-byte vectors.
 bool on_mfma(const PagedCall& c) {
     const int d = c.dim_qk;
-    return c.dtype != NATTEN_F32 && c.vec && d == c.cache.dim_v && (d == 32 || d == 64 || d == 96 || d == 128);
+    return c.vec && d == c.cache.dim_v && (d == 32 || d == 64 || d == 96 || d == 128);
 }
 
 PagedPlan plan(const PagedCall& c) {
@@ -925,7 +991,7 @@ PagedPlan plan(const PagedCall& c) {
     const long long rep = c.heads_q / c.heads_kv;
     const long long dil = c.dilation, classes = c.tokens < dil ? c.tokens : dil;
     const long long members = (c.tokens + dil - 1) / dil;
-    p.kind = !on_mfma(c) ? kRows : members * rep < kChunkFrom ? kFew : kChunk;
+    p.kind = !on_mfma(c) ? kRows : members * rep < kChunkFrom || c.dtype == NATTEN_F32 ? kFew : kChunk;
     const long long rows = p.rows = members * rep;
     if (p.kind == kChunk) {
         // 64 queries a wave where their accumulators leave two waves a SIMD
@@ -938,8 +1004,8 @@ PagedPlan plan(const PagedCall& c) {
     } else if (p.kind == kFew) {
         p.blocks = rows <= 16 ? 1 : rows <= 32 || c.dim_qk > 64 ? 2 : 4;
         p.M = kFewRows * p.blocks;
-        p.KT = 4 * kFewKeys;
-        p.least = 2;
+        p.KT = 4 * (c.dtype == NATTEN_F32 ? few_keys<float>() : few_keys<bf16>());
+        p.least = 256 / p.KT;
     } else {
         p.M = 4;
         p.KT = 64;
@@ -973,37 +1039,39 @@ PagedPlan plan(const PagedCall& c) {
 }
 
 // LDS of k_paged_few: the waves' values, then their results.
-template <int D>
+template <typename T, int D>
 constexpr size_t few_lds(int blocks) {
-    const size_t values = 4 * kFewKeys * row_elems<D>() * 2, results = 4 * kFewRows * blocks * D * sizeof(float);
+    const size_t values = 4 * few_keys<T>() * row_elems<D>() * sizeof(T), results = 4 * kFewRows * blocks * D * sizeof(float);
     return values > results ? values : results;
 }
 
 template <typename T, int D>
 hipError_t launch_mfma(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
     const dim3 grid(p.grid), block(kPagedThreads);
-    if (p.kind == kChunk) {
-        constexpr int lds = 2 * 2 * kChunkKeys * row_elems<D>() * sizeof(T);
-        if constexpr (D <= 64) {
-            if (p.blocks == 2)
-                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 2, 1>), grid, block, lds, s, a);
-            else
-                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 2>), grid, block, lds, s, a);
-        } else {
-            NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 1>), grid, block, lds, s, a);
+    if constexpr (!std::is_same<T, float>::value) {
+        if (p.kind == kChunk) {
+            constexpr int lds = 2 * 2 * kChunkKeys * row_elems<D>() * sizeof(T);
+            if constexpr (D <= 64) {
+                if (p.blocks == 2)
+                    NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 2, 1>), grid, block, lds, s, a);
+                else
+                    NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 2>), grid, block, lds, s, a);
+            } else {
+                NA_LAUNCH("na_paged_chunk", (k_paged_chunk<T, D, 1, 1>), grid, block, lds, s, a);
+            }
+            return hipGetLastError();
         }
-        return hipGetLastError();
     }
     if constexpr (D <= 64) {
         if (p.blocks == 4) {
-            NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 4>), grid, block, few_lds<D>(4), s, a);
+            NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 4>), grid, block, (few_lds<T, D>(4)), s, a);
             return hipGetLastError();
         }
     }
     if (p.blocks == 2)
-        NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 2>), grid, block, few_lds<D>(2), s, a);
+        NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 2>), grid, block, (few_lds<T, D>(2)), s, a);
     else
-        NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 1>), grid, block, few_lds<D>(1), s, a);
+        NA_LAUNCH("na_paged_few", (k_paged_few<T, D, 1>), grid, block, (few_lds<T, D>(1)), s, a);
     return hipGetLastError();
 }
 
@@ -1017,7 +1085,7 @@ hipError_t launch_kind(const PagedArgs& a, const PagedPlan& p, bool vec, hipStre
         else
             NA_LAUNCH("na_paged_rows", (k_paged_rows<T, 1>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
         e = hipGetLastError();
-    } else if constexpr (!std::is_same<T, float>::value) {
+    } else {
         if (a.Dqk == 32) e = launch_mfma<T, 32>(a, p, s);
         else if (a.Dqk == 64) e = launch_mfma<T, 64>(a, p, s);
         else if (a.Dqk == 96) e = launch_mfma<T, 96>(a, p, s);

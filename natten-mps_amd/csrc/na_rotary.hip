@@ -31,7 +31,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kUnits = 4;           // units of a thread in flight
 constexpr int kMaxTokens = 64;      // tokens per block
-constexpr int kMaxPairs = 128;      // turned pairs of a head (head dim 256)
 constexpr int kAngleFloats = 8192;  // LDS of cosines and sines per block
 
 struct RotaryArgs {

@@ -15,6 +15,8 @@ def get_support_matrix() -> dict:
             "fusion": {"na1d": True, "na2d": True, "na3d": True},
             "extras_allin1": {"na1d_qk_rpb": True, "na1d_av_fused": True, "na2d_qk_rpb": True,
                               "na2d_av_fused": True},
+            "rotary": {"rotary": True, "rotary_qk": True},
+            "paged": {"na1d_paged_append": True, "na1d_paged": True},
             "constraints": [
                 "Requires a ROCm GPU (gfx950 / MI355X) and the built libnatten_hip.so.",
                 "float32, float16 and bfloat16; head dims up to 256 (q/k and v may differ).",
@@ -24,6 +26,8 @@ def get_support_matrix() -> dict:
                 "An even kernel equal to a non-causal, undilated axis length is rejected.",
                 "Variable-length (na{1,2,3}d_varlen): one launch per op for the whole padded batch, "
                 "fused backward; padding positions are zero.",
+                "Rotary positions (rotary, rotary_qk): forward and gradients, 1-3 axes.",
+                "Paged cache (na1d_paged_append, na1d_paged): causal 1-D attention, no gradients.",
             ],
         },
     }

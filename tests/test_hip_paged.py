@@ -144,6 +144,10 @@ CASES = {
     "long": ([(1, 20000), (1, 100)], 8, 1, 64, 64, None, 1, BF),
     "long_drafts_fp32": ([(2, 5000)], 2, 1, 32, 16, None, 1, F32),
     "many_sequences": ([(1, 1 + (37 * i) % 90) for i in range(300)], 2, 1, 64, 16, None, 1, BF),
+    "chunk_fp32_dim128": ([(130, 200), (7, 300)], 6, 2, 128, 24, None, 1, F32),
+    "chunk_fp32_dim96": ([(41, 90), (7, 30)], 4, 2, 96, 16, 25, 1, F32),
+    "drafts_fp32": ([(5, 700), (3, 64), (1, 1), (4, 4)], 8, 2, 64, 16, None, 1, F32),
+    "token_fp32_dim96": ([(1, 300), (1, 17)], 3, 3, 96, 8, 50, 3, F32),
     "many_heads_rep3": ([(11, 260)], 9, 3, 128, 16, None, 1, FP),
 }
 

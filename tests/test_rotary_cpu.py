@@ -187,7 +187,8 @@ def _paged(**over):
     (dict(pages=0), 1, "pages"), (dict(page_size=0), 1, "page_size"), (dict(table_width=0), 1, "table_width"),
     (dict(table_stride=-1), 1, "stride"), (dict(key_stride=(-1, 1, 1)), 1, "stride"), (dict(kernel=-1), 1, "kernel"),
     (dict(dilation=0), 1, "dilation"), (dict(dilation=2), 1, "needs a kernel"),
-    (dict(batch=2 ** 20, tokens=2 ** 20), 2, "2\\^30"),
+    (dict(batch=2 ** 20, tokens=2 ** 20), 2, "2\\^27"), (dict(batch=2 ** 16, tokens=2 ** 12), 2, "2\\^27"),
+    (dict(table_width=2 ** 20, page_size=2 ** 11), 2, "positions"),
 ])
 def test_paged_codes(over, code, text):
     import re
