@@ -148,6 +148,14 @@ CASES = {
     "chunk_fp32_dim96": ([(41, 90), (7, 30)], 4, 2, 96, 16, 25, 1, F32),
     "drafts_fp32": ([(5, 700), (3, 64), (1, 1), (4, 4)], 8, 2, 64, 16, None, 1, F32),
     "token_fp32_dim96": ([(1, 300), (1, 17)], 3, 3, 96, 8, 50, 3, F32),
+    "chunk_wide": ([(70 - i % 7, 75 + (13 * i) % 90) for i in range(64)], 8, 8, 64, 16, None, 1, BF),
+    "chunk_wide_window": ([(70 - i % 7, 75 + (13 * i) % 90) for i in range(64)], 8, 8, 32, 8, 21, 1, FP),
+    "chunk_long": ([(70, 5000), (64, 2500), (3, 9)], 4, 2, 64, 16, None, 1, BF),
+    "chunk_long_dim128": ([(70, 5000), (64, 2500)], 4, 2, 128, 64, 4500, 1, FP),
+    "ragged_many": ([(1, 9000)] + [(1, 1 + (37 * i) % 90) for i in range(299)], 2, 1, 64, 64, None, 1, BF),
+    "odd_dim_long": ([(2, 3000), (1, 700)], 2, 1, 20, 16, None, 1, BF),
+    "long_drafts_dilated": ([(20, 9000), (17, 40)], 4, 2, 32, 16, 4000, 2, BF),
+    "long_fp32_rows": ([(20, 3000), (9, 100)], 4, 2, 64, 16, None, 1, F32),
     "many_heads_rep3": ([(11, 260)], 9, 3, 128, 16, None, 1, FP),
 }
 
@@ -229,6 +237,45 @@ def test_nonfinite_outside_the_window(new, kernel, dil, dtype):
             t[~used.to(DEV)] = bad
         got = p.run(kernel, dil)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_nonfinite_in_cut_and_wide_calls(dtype):
+    """As above where keys are cut into parts (few rows and many) and on tall
+    tiles of many sequences: unused slots and keys behind every window."""
+    for rows, hq, hkv, kernel in (([(5, 6000)], 4, 2, 3000), ([(70, 6000)], 4, 2, 3000), ([(2, 6000)], 4, 2, None),
+                                  ([(70, 110)] * 64, 8, 8, 20)):
+        p = Problem(rows, hq, hkv, 64, 16, dtype, spare=3)
+        want = p.run(kernel)
+        new, length = rows[0]
+        first = 0 if kernel is None else max(0, length - new - kernel + 1)
+        used = torch.zeros(p.kp.shape[:2], dtype=torch.bool, device=DEV)
+        for b in range(len(rows)):
+            keys = torch.arange(first, length, device=DEV)
+            used[p.table[b, keys // 16].long(), keys % 16] = True
+        for bad in (math.nan, math.inf):
+            p.kp[~used] = bad
+            p.vp[~used] = bad
+            # within the used ones: the first key, seen by the first new token only
+            if kernel is not None:
+                for b in range(len(rows)):
+                    p.vp[p.table[b, first // 16].long(), first % 16] = bad
+            got = p.run(kernel)
+            rest = slice(0, None) if kernel is None else slice(1, None)
+            assert torch.isfinite(got[0][:, rest]).all()
+            if kernel is None:
+                assert torch.equal(got[0], want[0])
+            else:
+                # rows of a redone tile sum in another order: each of the two
+                # is within the module's bound of the exact value, whose
+                # magnitudes are at most max |v| and the product of norms
+                norms = p.q.float().norm(dim=-1).max() * p.kp[used].float().norm(dim=-1).max() * 64 ** -0.5
+                v = p.vp[used].float()
+                top = v[torch.isfinite(v)].abs().max()
+                step = torch.finfo(dtype).eps / 2
+                rel = (8 + length ** 0.5 + 2 * (64 + 4) * norms) * 2.0 ** -24 + (step if dtype == BF else 0) + step
+                assert ((got[0] - want[0])[:, rest].float().abs() <= 2 * rel * top).all()
+            assert torch.equal(got[1], want[1])
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
