@@ -67,7 +67,10 @@ __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -
 // ---------------------------------------------------------------------------
 
 // A wave per row; lanes take 64 keys for the scores, then 64 head dims for
-// the products.  `VEC` elements of a key are read at once.
+// the products.  `VEC` elements of a key are read at once.  Head dims and
+// alignments that the MFMA kernels do not take; a row's keys are read once a
+// query head, and address arithmetic bounds it (fp32, 257 tokens in a window
+// of 63, 4 heads of 32: 19 us where k_paged_few takes 11).
 template <typename T, int VEC>
 __global__ __launch_bounds__(kPagedThreads) void k_paged_rows(PagedArgs a) {
     __shared__ float qs[4][256];
@@ -237,7 +240,11 @@ __device__ __forceinline__ bool four_nonfinite(f32x4_t x) { return item_nonfinit
 //
 // Each key is read once per kv head and nothing else is big, so HBM bounds
 // it: the next keys' loads are issued as soon as the registers are free, and
-// page numbers one step before that.
+// page numbers one step before that.  32 requests of 1 to 16385 tokens, 32/8
+// heads of 128, one new token each: 1.08 GB in 231 to 240 us (4.6 TB/s; a
+// large copy moves 4.95), in fp32 420 us (5.1 TB/s).  One request of 131070
+// tokens and 5 new ones, 8/1 heads of 64: 34 MB in 19 us, of which 11 are
+// there with 600 tokens too: latency of lengths, pages, keys and parts.
 //
 // fp32 takes v_mfma 16x16x4, 16 keys at a time: element e of the 16-byte
 // pieces is one product's k slot (both operands permuted alike), and a lane's
@@ -556,6 +563,14 @@ __device__ __forceinline__ float other_half(float v) {
 // probabilities are the second product's operand as they lie: of the 16
 // accumulators of a 32-key block, half-wave h holds keys 8 (i / 4) + 4 h +
 // i % 4, and the values' operand is read (transposed) in that order.
+//
+// 4096 tokens over 32096 keys, 16/4 heads of 128, two requests: 1.89 to 2.2 ms
+// (735 to 860 TFLOP/s; a large matrix product reaches 1257 on this card, both
+// at the clock that power leaves).  Products keep the matrix cores 39 % busy
+// and the softmax the vector ALUs 45 %; the two waves of a SIMD wait for LDS
+// reads and the barrier of a tile in the rest.  DEPTH 2 keeps two tiles'
+// loads in flight, for tiles of one block, whose step is shorter than a trip
+// to memory.
 constexpr int kChunkKeys = 64;
 
 template <typename T, int D, int QB, int DEPTH>
@@ -958,8 +973,16 @@ __global__ __launch_bounds__(WIDE ? kJoinThreads : kPagedThreads) void k_paged_j
 // Workgroups aimed at when the tiles are few: two a compute unit.
 constexpr int kTarget = 512;
 
-// Rows of a class from which the tall tiles are taken.
-constexpr int kChunkFrom = 64;
+// Rows of cut tiles up to which a workgroup joins each (k_paged_join WIDE);
+// more take a group of lanes each.  Tiles x rows, WIDE / not, us: 32 x 4 5 /
+// 11, 64 x 12 5 / 8, 256 x 4 5 / 5, 64 x 64 12 / 8, 64 x 128 20 / 8.
+constexpr unsigned kWideRows = 1024;
+
+// Rows of a class up to which k_paged_few takes them on one read of the keys;
+// more take the tall tiles.  32 requests over up to 16384 keys, few / chunk
+// kernel with their joins, us: heads of 128, 32 rows 256 / 266, 64 rows 429 /
+// 286; heads of 64, 32 rows 40 / 53, 64 rows 51 / 55, 96 rows 77 / 58.
+constexpr int few_rows(int dim) { return dim <= 64 ? 64 : 32; }
 
 enum PagedKind { kRows, kFew, kChunk };
 
@@ -991,17 +1014,23 @@ PagedPlan plan(const PagedCall& c) {
     const long long rep = c.heads_q / c.heads_kv;
     const long long dil = c.dilation, classes = c.tokens < dil ? c.tokens : dil;
     const long long members = (c.tokens + dil - 1) / dil;
-    p.kind = !on_mfma(c) ? kRows : members * rep < kChunkFrom || c.dtype == NATTEN_F32 ? kFew : kChunk;
+    p.kind = !on_mfma(c) ? kRows : members * rep <= few_rows(c.dim_qk) || c.dtype == NATTEN_F32 ? kFew : kChunk;
     const long long rows = p.rows = members * rep;
     if (p.kind == kChunk) {
         // 64 queries a wave where their accumulators leave two waves a SIMD
-        // and the tiles still fill the device
+        // and the tiles still fill the device: half the reads of LDS for each
+        // product (2048 tokens in a window of 1025, heads of 64, one / two
+        // blocks: 8 requests, 512 tall tiles, 72 / 64 us; 4 requests 41 / 44)
         const long long tall = classes * ((rows + 255) / 256) * c.batch * c.heads_kv;
         p.blocks = c.dim_qk <= 64 && tall >= kTarget ? 2 : 1;
         p.M = 128 * p.blocks;
         p.KT = kChunkKeys;
+        // 2048 keys: parts of 128 rows and their join cost as much as 1000
+        // keys take (17 blocks whole 42 us, in two parts 32 + 9)
         p.least = 32;
     } else if (p.kind == kFew) {
+        // one read of the keys for all rows, if the registers hold them (40
+        // rows of 64 dims: 19 us, as three tiles of 16 23)
         p.blocks = rows <= 16 ? 1 : rows <= 32 || c.dim_qk > 64 ? 2 : 4;
         p.M = kFewRows * p.blocks;
         p.KT = 4 * (c.dtype == NATTEN_F32 ? few_keys<float>() : few_keys<bf16>());
@@ -1094,13 +1123,14 @@ hipError_t launch_kind(const PagedArgs& a, const PagedPlan& p, bool vec, hipStre
     if (e != hipSuccess || !p.split) return e;
     const unsigned tiles = static_cast<unsigned>(p.tiles < kTarget ? p.tiles : kTarget);
     const unsigned rows = static_cast<unsigned>(std::min<long long>(p.M, p.rows));
-    if (p.kind == kChunk) {
-        const unsigned groups = kPagedThreads / (a.Dv / 4);
+    if (tiles * rows > kWideRows) {
+        const unsigned groups = kPagedThreads / ((a.Dv + 3) / 4);
         NA_LAUNCH("na_paged_join", (k_paged_join<T, false>), dim3(tiles, (rows + groups - 1) / groups),
                   dim3(kPagedThreads), 0, s, a);
     } else {
-        // parts per tile go as one over the tiles: enough groups of lanes
-        // that each joins a handful
+        // the fewer the tiles, the more parts has each: groups of lanes
+        // enough that each joins a handful (513 parts of one tile: 15 us with
+        // 256 threads, 6 with 1024; 256 tiles of 4 rows, 9 parts: 5 and 11)
         const int threads = tiles <= 16 ? kJoinThreads : kPagedThreads;
         NA_LAUNCH("na_paged_join", (k_paged_join<T, true>), dim3(tiles, rows), dim3(threads), 0, s, a);
     }

@@ -19,7 +19,12 @@
 // The op reads and writes each element once, so memory bounds it.  A block
 // takes `tb` consecutive tokens: it computes their cosines and sines into
 // LDS once for all heads, then walks the tokens' vectors in memory order
-// (lanes on consecutive 16-byte vectors).
+// (lanes on consecutive 16-byte vectors), its first loads out before the
+// angles.  4 x 16384 tokens of 8/2 heads of 64, bf16: 31 us (5.4 TB/s); 64 x
+// 56 x 56 of 4/4 heads of 32, interleaved fp16 views: 34 us (6.1 TB/s); three
+// axes of 16 dims, 32768 tokens of 8/8 heads of 64: 31 us (4.4 TB/s); 4096
+// tokens of 4 prompts, 32/8 heads of 128, into pages: 52 us (4.8 TB/s).  A
+// large copy moves 4.95 TB/s.
 #include <type_traits>
 
 #include "na_launch.h"
