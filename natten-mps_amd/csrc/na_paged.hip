@@ -467,7 +467,7 @@ __global__ __launch_bounds__(kPagedThreads, few_waves<T>(D, NB)) void k_paged_fe
     }
     // the four waves' parts, through the LDS that held their values
     float* const parts = reinterpret_cast<float*>(lds);  // [4][rows][D]
-    __syncthreads();
+    lds_publish_barrier();
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         float* const ow = parts + (wave * kRowsOf + 16 * n + col) * D;
@@ -941,7 +941,7 @@ __global__ __launch_bounds__(WIDE ? kJoinThreads : kPagedThreads) void k_paged_j
                 j.add(p[0], p[1], f32x4_t{p[2], p[3], p[4], p[5]});
             }
         }
-        __syncthreads();
+        lds_publish_barrier();
         if (g < 8) {
             o[tid][0] = j.m;
             o[tid][1] = j.l;

@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
             coord[t][2] = i2;
         }
     }
-    __syncthreads();
+    lds_publish_barrier();
 
     // The block's first loads go out before its angles are computed.
     using R = raw_t<T, VEC>;
