@@ -30,20 +30,13 @@ own = False
 _DEV = "cuda"
 
 
-_na = None
-
-
 def _package():
-    """The package, looked up once: a program imports it at its top."""
-    global _na
-    if _na is not None:
-        return _na
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "natten-mps_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
-    import natten_mps_amd as _na
+    import natten_mps_amd
 
-    return _na
+    return natten_mps_amd
 
 
 _ROTARY = dict(op="rotary", dtype="bfloat16", batch=1, size="128", heads=4, kv_heads=4, dim=32, turned=32,
