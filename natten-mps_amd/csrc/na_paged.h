@@ -87,6 +87,13 @@ __device__ __forceinline__ SeqGeo seq_geo(const PagedArgs& a, int n, int len) {
     return g;
 }
 
+// First key (class coordinates) of the window of the query at w: K - 1 keys
+// behind it, not below 0.  w may lie before the sequence (down to -2^27) and
+// K be any int, whose difference passes 32 bits: compared, not subtracted.
+__device__ __forceinline__ int first_key(const PagedArgs& a, int w) {
+    return a.K && w >= a.K ? w - a.K + 1 : 0;
+}
+
 // A workgroup's share: keys [u_lo, u_hi] (class coordinates) of one tile.
 struct Share {
     int b, h, cls, c;         // class: its first token, its residue
@@ -240,7 +247,7 @@ __device__ __forceinline__ bool find_share(const PagedArgs& a, Share& r) {
     r.u_hi = -1;
     if (r.rows > 0) {
         const int wf = r.w0 + fdiv(r.row0, a.frep), wl = r.w0 + fdiv(r.row0 + r.rows - 1, a.frep);
-        r.u_lo = a.K ? imax(0, wf - a.K + 1) : 0;
+        r.u_lo = first_key(a, wf);
         r.u_hi = imin(wl, r.c < a.cap ? fdiv(a.cap - 1 - r.c, a.fdil) : -1);
     }
     if (r.split) {

@@ -87,7 +87,7 @@ __global__ __launch_bounds__(kPagedThreads) void k_paged_rows(PagedArgs a) {
     // the wave reads its own part of qs only
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const int w = r.w0 + fdiv(r.row0 + wave, a.frep);
-    const int lo = imax(r.u_lo, a.K ? w - a.K + 1 : 0), hi = imin(r.u_hi, w);
+    const int lo = imax(r.u_lo, first_key(a, w)), hi = imin(r.u_hi, w);
     const int* const table = a.table + r.b * a.table_stride;
     const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh;
     const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh;
@@ -211,7 +211,7 @@ __device__ __forceinline__ f32x4_t exact_four(const PagedArgs& a, const Share& r
     const int* const table = a.table + r.b * a.table_stride;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (int u = imax(r.u_lo, a.K ? w - a.K + 1 : 0); u <= imin(r.u_hi, w); ++u) {
+    for (int u = imax(r.u_lo, first_key(a, w)); u <= imin(r.u_hi, w); ++u) {
         int page, slot;
         if (!key_at(a, table, r.c, u, r.u_hi, page, slot)) continue;
         const T* const k = static_cast<const T*>(a.k) + (page * a.kp + slot * a.ks + r.h * a.kh);
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(kPagedThreads, few_waves<T>(D, NB)) void k_paged_fe
         hi[n] = r.w0 + fdiv(r.row0 + imin(16 * n + col, r.rows - 1), a.frep);
     }
     const int all_hi = imin(r.w0 + fdiv(r.row0, a.frep), r.u_hi);
-    const int all_lo = a.K ? r.w0 + fdiv(r.row0 + r.rows - 1, a.frep) - a.K + 1 : 0;
+    const int all_lo = first_key(a, r.w0 + fdiv(r.row0 + r.rows - 1, a.frep));
     const int steps = (r.u_hi - r.u_lo + KS) / KS;  // 0 when empty: u_hi = u_lo - 1 at least
     const int* const table = a.table + r.b * a.table_stride;
     const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh + E * g;
@@ -611,7 +611,7 @@ __global__ __launch_bounds__(kPagedThreads, DEPTH == 2 ? 3 : 2) void k_paged_chu
     // what some and what all rows of the wave see
     const int wf = r.w0 + fdiv(r.row0 + imin(wrow, r.rows - 1), a.frep);
     const int wl = r.w0 + fdiv(r.row0 + imin(wrow + 32 * QB, r.rows) - 1, a.frep);
-    const int some_lo = a.K ? wf - a.K + 1 : 0, all_lo = a.K ? wl - a.K + 1 : 0;
+    const int some_lo = first_key(a, wf), all_lo = first_key(a, wl);
     const bool idle = wrow >= r.rows;
     const int steps = (r.u_hi - r.u_lo + kChunkKeys) / kChunkKeys;
 
