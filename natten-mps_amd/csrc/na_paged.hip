@@ -493,7 +493,8 @@ __global__ __launch_bounds__(kPagedThreads, few_waves<T>(D, NB)) void k_paged_fe
             lt = fmaf(wt, ml[w][rw][1], lt);
             x += wt * *reinterpret_cast<const f32x4_t*>(parts + (w * kRowsOf + rw) * D + d);
         }
-        if (four_nonfinite(x) && !item_nonfinite(mt) && !item_nonfinite(lt)) x = exact_four<T, D>(a, r, rw, mt, d);
+        if (lt == 0.f) x = f32x4_t{0.f, 0.f, 0.f, 0.f};  // no key: 0 times what others see is not 0 if it is not finite
+        else if (four_nonfinite(x) && !item_nonfinite(mt) && !item_nonfinite(lt)) x = exact_four<T, D>(a, r, rw, mt, d);
         if (r.split) {
             const long long at = static_cast<long long>(r.index) * kRowsOf + rw;
             *reinterpret_cast<f32x4_t*>(a.part + at * D + d) = x;
@@ -859,11 +860,12 @@ __global__ __launch_bounds__(kPagedThreads, DEPTH == 2 ? 3 : 2) void k_paged_chu
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) total += o[b][t][i];
-        if (item_nonfinite(total) && !item_nonfinite(m[b]) && !item_nonfinite(lt)) {
-            // written over, four head dims at a time
+        if (item_nonfinite(total) && (lt == 0.f || (!item_nonfinite(m[b]) && !item_nonfinite(lt)))) {
+            // written over, four head dims at a time; zeros where the row has no key
 #pragma unroll 1
             for (int d = 4 * h; d < D; d += 8) {
-                const f32x4_t x = exact_four<T, D>(a, r, rw, m[b], d);
+                f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+                if (lt != 0.f) x = exact_four<T, D>(a, r, rw, m[b], d);
                 if (r.split)
                     *reinterpret_cast<f32x4_t*>(a.part + (static_cast<long long>(r.index) * a.M + rw) * D + d) = x;
                 else

@@ -1,14 +1,107 @@
-"""Attention over a paged cache where its arithmetic has edges: windows of any
-length beside tokens before the sequence.  Tolerances are those of
+"""Attention over a paged cache where its arithmetic has edges: values that are
+not finite beside rows that do not attend to them, and windows of any length
+beside tokens before the sequence.  Tolerances are those of
 ``test_hip_paged``."""
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
 
-from test_hip_paged import BF, DEV, F32, Problem, check
+from test_hip_paged import BF, DEV, F32, FP, Problem, check
 
 pytestmark = pytest.mark.gpu
+
+
+def _at(p, seq, pos):
+    """Page and slot of a position."""
+    return p.table[seq, pos // p.page].long(), pos % p.page
+
+
+def exact_rows(p, seq, tokens, kernel=None, dilation=1):
+    """(out, lse, sum of p |v| over finite values, largest score error per
+    unit 2^-24) of some of a sequence's new tokens, in float64 on the CPU.
+    A value that is not finite comes out as itself wherever a key that the
+    token attends to holds it."""
+    n, length = p.news[seq].item(), p.lens[seq].item()
+    have = torch.arange(length)
+    pages = p.table[seq].cpu().long()[have // p.page]
+    have = have[pages >= 0]
+    pages = pages[pages >= 0]
+    k, v = (t.cpu()[pages, have % p.page].double() for t in (p.kp, p.vp))
+    H, D = p.q.shape[2:]
+    rep = H // p.hkv
+    res = []
+    for i in tokens:
+        back = length - n + i - have
+        ok = back >= 0
+        if kernel is not None:
+            ok &= (back % dilation == 0) & (back < kernel * dilation)
+        ki, vi = k[ok].repeat_interleave(rep, 1), v[ok].repeat_interleave(rep, 1)
+        q = p.q[seq, i].cpu().double()
+        s = (ki * q).sum(-1) * D ** -0.5
+        w = s.softmax(0)[..., None] if len(s) else torch.zeros(0, H, 1, dtype=torch.float64)
+        res.append(((w * vi).sum(0), s.logsumexp(0) if len(s) else torch.full((H,), -math.inf, dtype=torch.float64),
+                    (w * torch.where(vi.isfinite(), vi.abs(), 0)).sum(0),
+                    (ki.abs() * q.abs()).sum(-1).amax(0) * D ** -0.5 if len(s) else torch.zeros(H, dtype=torch.float64)))
+    return [torch.stack(x) for x in zip(*res)]
+
+
+def check_rows(got, p, seq, tokens, kernel=None, dilation=1, slack=0.0, what=""):
+    """The bound of ``test_hip_paged.check`` at finite results, the others
+    exactly."""
+    want, wlse, mag, err = exact_rows(p, seq, tokens, kernel, dilation)
+    out, lse = (t[seq, list(tokens)].cpu() for t in got)
+    step = torch.finfo(out.dtype).eps / 2
+    n = max(p.lens[seq].item(), 1)
+    sums = (8 + n ** 0.5) * 2.0 ** -24
+    delta = (p.q.shape[-1] + 4) * 2.0 ** -24 * err
+    probs = 0.0 if out.dtype == F32 else step
+    fin = want.isfinite()
+    bound = step * want.abs() + (probs + sums + 2 * delta[..., None]) * mag * 1.01 + slack
+    bound += torch.finfo(out.dtype).tiny * torch.finfo(out.dtype).eps
+    diff = (out.double() - want).abs()
+    assert torch.isfinite(out[fin]).all(), f"{what}: {(~torch.isfinite(out[fin])).sum()} results are not finite"
+    worst = (diff - bound)[fin].max().item() if fin.any() else 0.0
+    assert worst <= 0, f"{what}: {diff[fin].max().item():.3g} off, {worst:.3g} past its bound"
+    assert torch.equal(out.double()[~fin].nan_to_num(nan=7.0), want[~fin].nan_to_num(nan=7.0)), f"{what}: not finite"
+    empty = wlse == -math.inf
+    assert torch.equal(lse == -math.inf, empty) and (out[empty] == 0).all(), f"{what}: rows without keys"
+    d = (lse.double() - wlse)[~empty].abs() - (delta + sums + 4 * 2.0 ** -24 * (1 + wlse.abs()))[~empty]
+    assert d.numel() == 0 or d.max().item() <= 0, f"{what}: lse"
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("new, length, hq, hkv", [
+    (5, 5890, 4, 2),     # parts of 256 keys, two keys in the last: few rows
+    (70, 65537, 2, 1),   # parts of 2048 keys, one key in the last: many rows
+])
+def test_rows_without_a_key_in_a_part(new, length, hq, hkv, bad, dtype):
+    """Keys are cut and the last part holds the newest keys alone: a value
+    there that is not finite stays with the tokens that attend to it."""
+    p = Problem([(new, length)], hq, hkv, 32 if hkv == 1 else 64, 64, dtype)
+    p.vp[_at(p, 0, length - 1)] = bad
+    got = p.run()
+    check_rows(got, p, 0, sorted({0, 1, new // 2, new - 2, new - 1}))
+    assert torch.isfinite(got[0][0, :new - 1]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("new, hq", [(8, 2), (8, 8), (70, 4)])
+def test_rows_without_a_key_beside_others(new, hq, dtype):
+    """Tokens whose pages are all absent are empty, whatever the values of
+    the tokens beside them hold."""
+    p = Problem([(new, 200)], hq, 2, 64, 4, dtype)
+    first = 200 - new
+    gone = [j // 4 for j in range(first - 1, 196)]
+    p.table[0, gone] = -1
+    for j, bad in ((196, math.inf), (198, math.nan), (199, -math.inf)):
+        p.vp[_at(p, 0, j)[0], j % 4, :, 3:] = bad
+    got = p.run(2)
+    check_rows(got, p, 0, range(new), 2)
+    assert (got[1][0, :196 - first] == -math.inf).all()
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
