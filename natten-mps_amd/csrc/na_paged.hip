@@ -198,35 +198,39 @@ __device__ __forceinline__ uint4 scaled(uint4 x, const ScaleParts& s) {
                       (x.w & s.keep) ^ s.flip);
 }
 
-// Four head dims of a row, key by key in plain arithmetic: where a value that
-// is not finite met a probability of 0 in a product, rows of the tile that do
-// not attend to that key got NaN.  Keys that the row does not attend to are
-// not touched here.  Not normalised; m the row's maximum (base 2).
-template <typename T, int D>
-__device__ __forceinline__ f32x4_t exact_four(const PagedArgs& a, const Share& r, int row, float m, int d) {
-    int qi, qh;
-    row_token(a, r.cls, r.h, r.row0 + row, qi, qh);
-    const T* const q = static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
-    const int w = r.w0 + fdiv(r.row0 + row, a.frep);
-    const int* const table = a.table + r.b * a.table_stride;
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-    for (int u = imax(r.u_lo, first_key(a, w)); u <= imin(r.u_hi, w); ++u) {
-        int page, slot;
-        if (!key_at(a, table, r.c, u, r.u_hi, page, slot)) continue;
-        const T* const k = static_cast<const T*>(a.k) + (page * a.kp + slot * a.ks + r.h * a.kh);
-        const T* const v = static_cast<const T*>(a.v) + (page * a.vp + slot * a.vs + r.h * a.vh) + d;
-        float dot = 0.f;
-#pragma unroll 1
-        for (int x = 0; x < D; ++x) dot = fmaf(to_f(q[x]), to_f(k[x]), dot);
-        const float p = __builtin_amdgcn_exp2f(dot * (a.scale * kLog2e) - m);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = fmaf(p, to_f(v[i]), acc[i]);
-    }
-    return acc;
-}
+// A product adds 0 times the values that a row does not attend to, which is
+// NaN where such a value is not finite.  Rows with a NaN are summed again
+// (redo_rows), in walks whose products meet finite values only; an infinity
+// in a result is the row's own.
+enum RedoWalk {
+    kFinite,  // values that are not finite count as 0
+    kPlus,    // +infinity and NaN as 1, the rest as 0, keys attended to as 1
+    kMinus,   // -infinity and NaN
+    kWalks
+};
 
-__device__ __forceinline__ bool four_nonfinite(f32x4_t x) { return item_nonfinite((x[0] + x[1]) + (x[2] + x[3])); }
+// The elements of a vector of values as a walk takes them.
+template <typename T>
+__device__ __forceinline__ uint4 walk_values(uint4 x, int walk) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr uint32_t kOne = F32 ? 0x3F800000u : Mma<typename std::conditional<F32, bf16, T>::type>::kOnes & 0xffffu;
+    constexpr uint32_t kSign = F32 ? 0x80000000u : 0x8000u;
+    constexpr uint32_t kInf = F32 ? 0x7F800000u : std::is_same<T, f16>::value ? 0x7C00u : 0x7F80u;
+    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int sh = 0; sh < 32; sh += 8 * static_cast<int>(sizeof(T))) {
+            const uint32_t e = F32 ? w[i] : (w[i] >> sh) & 0xffffu, mag = e & (kSign - 1);
+            const bool plus = mag > kInf || e == kInf, minus = mag > kInf || e == (kInf | kSign);
+            const uint32_t v = walk == kFinite ? (mag < kInf ? e : 0u) : (walk == kPlus ? plus : minus) ? kOne : 0u;
+            r |= v << sh;
+        }
+        w[i] = r;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // 16 NB rows, the four waves on different keys, 32 at a time each.
 //
@@ -272,6 +276,173 @@ constexpr int few_waves(int dim, int blocks) {
     return blocks > 1 || dim > 96 ? 2 : dim > 64 ? 3 : 4;
 }
 
+// Where a row's results go: a part, or the output with its sum.
+template <typename T>
+__device__ __forceinline__ void put_four(const PagedArgs& a, const Share& r, int row, int d, f32x4_t x, float l) {
+    if (r.split) {
+        *reinterpret_cast<f32x4_t*>(a.part + (static_cast<long long>(r.index) * a.M + row) * a.Dv + d) = x;
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    int i, hq;
+    row_token(a, r.cls, r.h, r.row0 + row, i, hq);
+    T* const out = static_cast<T*>(a.out) + r.b * a.lo.b + i * a.lo.s2 + hq * a.lo.h + d;
+    if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<f32x4_t*>(out) = x * inv;
+    else
+        *reinterpret_cast<uint2*>(out) = make_uint2(Mma<T>::pack(x[0] * inv, x[1] * inv),
+                                                    Mma<T>::pack(x[2] * inv, x[3] * inv));
+}
+
+// Rows of the tile that are summed again, 16 at a time, the waves on
+// different keys as in k_paged_few: `again(row, m, l)` says which, and gives
+// their maximum and sum (the scores do not depend on the values, so both hold
+// as they are).  A walk over the finite values gives the sums, two more
+// whether the row attends to infinities of either sign or NaN.  Three walks
+// for 16 rows, whatever the values hold: latency bounds them, since one
+// workgroup redoes its tile alone and loads nothing ahead.  A pass with finite
+// values / a NaN at the newest token / one that all rows attend to, heads of
+// 128, us: 4 tokens over 2000 keys 18 / 49 / 49, 512 tokens 60 / 480 / 1720,
+// 4096 tokens over 32096 keys 2250 / 39400 / 65800.
+// All of the workgroup's threads come here, the tile's own LDS is free.
+template <typename T, int D, class Again>
+__device__ __forceinline__ void redo_rows(const Share& r, unsigned char* lds, const Again& again) {
+    const PagedArgs& a = *static_cast<const PagedArgs*>(kernargs());  // read afresh: nothing is kept for this path
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int E = 16 / sizeof(T), C = D / (4 * E);
+    constexpr int LD = row_elems<D>(), DB = D / 16, KS = few_keys<T>(), KB = KS / 16;
+    constexpr int kQuads = D / 4, kItems = (16 * kQuads + kPagedThreads - 1) / kPagedThreads;
+    const int tid = opaque(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int col = lane & 15, g = lane >> 4;
+    const ScaleParts sp = scale_parts<T>(a.scale);
+    const int* const table = a.table + r.b * a.table_stride;
+    const T* const kb = static_cast<const T*>(a.k) + r.h * a.kh + E * g;
+    const T* const vb = static_cast<const T*>(a.v) + r.h * a.vh + E * g;
+    T* const X = reinterpret_cast<T*>(lds) + wave * (KS * LD);
+    float* const parts = reinterpret_cast<float*>(lds);  // [4][16][D]
+    const uint32_t reach = a.K ? a.K - 1 : 0x7fffffffu;
+    lds_publish_barrier();
+#pragma unroll 1
+    for (int row0 = 0; row0 < r.rows; row0 += 16) {
+        const int last = imin(row0 + 15, r.rows - 1), row = imin(row0 + col, last);
+        float m, l;
+        if (!__ballot(again(row, m, l))) continue;  // the same in every wave
+        const float ref = m == -INFINITY ? 0.f : m;
+        int qi, qh;
+        row_token(a, r.cls, r.h, r.row0 + row, qi, qh);
+        const T* const q = static_cast<const T*>(a.q) + r.b * a.lq.b + qi * a.lq.s2 + qh * a.lq.h;
+        uint4 qf[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) qf[c] = scaled(*reinterpret_cast<const uint4*>(q + E * (4 * c + g)), sp);
+        const int hi = r.w0 + fdiv(r.row0 + row, a.frep);
+        const int lo_u = imax(r.u_lo, first_key(a, r.w0 + fdiv(r.row0 + row0, a.frep)));
+        const int hi_u = imin(r.u_hi, r.w0 + fdiv(r.row0 + last, a.frep));
+        f32x4_t sum[kItems];
+        uint32_t plus[kItems];
+#pragma unroll 1
+        for (int walk = kFinite; walk < kWalks; ++walk) {
+            f32x4_t o[DB];
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int ub = lo_u + wave * KS; ub <= hi_u; ub += 4 * KS) {
+                f32x4_t s[KB];
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    int page = 0, slot = 0;
+                    const bool ok = key_at(a, table, r.c, ub + 16 * b + col, hi_u, page, slot);
+                    // keys that are not there: the pool's first slot, masked below
+                    const int pg = ok ? page : 0, sl = ok ? slot : 0;
+                    const T* const k = kb + (pg * a.kp + sl * a.ks);
+                    const T* const v = vb + (pg * a.vp + sl * a.vs);
+                    s[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    const int rw = 16 * b + col, sw = few_swz<T, D>(rw);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const uint4 kf = *reinterpret_cast<const uint4*>(k + 4 * E * c);
+                        uint4 vf = *reinterpret_cast<const uint4*>(v + 4 * E * c);
+                        if constexpr (F32) {
+                            const f32x4v_t x = __builtin_bit_cast(f32x4v_t, kf), y = __builtin_bit_cast(f32x4v_t, qf[c]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                s[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], s[b], 0, 0, 0);
+                        } else {
+                            s[b] = Mma<T>::run(kf, qf[c], s[b]);
+                        }
+                        vf = walk_values<T>(vf, walk);
+                        if (!ok) vf = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(X + rw * LD + ((4 * c + g) ^ sw) * E) = vf;
+                    }
+                    const uint32_t have = static_cast<uint32_t>(__ballot(ok)) >> (4 * g);
+                    const uint32_t back = static_cast<uint32_t>(hi - ub - 16 * b - 4 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool seen = back - i <= reach && ((have >> i) & 1) && s[b][i] != -INFINITY;
+                        const float p = walk == kFinite ? __builtin_amdgcn_exp2f(fmaf(s[b][i], sp.sc2, -ref)) : 1.f;
+                        s[b][i] = seen ? p : 0.f;
+                    }
+                }
+                if constexpr (F32) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int rw = 4 * g + i;
+#pragma unroll
+                        for (int db = 0; db < DB; ++db) {
+                            const float x = X[rw * LD + ((4 * db + (col >> 2)) ^ few_swz<T, D>(rw)) * 4 + (col & 3)];
+                            o[db] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, s[0][i], o[db], 0, 0, 0);
+                        }
+                    }
+                } else {
+                    const uint4 p = pack8<T>(s);
+                    const int r0 = 4 * g + (col >> 2), r1 = 16 + r0;
+                    const int s0 = piece_swz<D>(r0), s1 = piece_swz<D>(r1);
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        const int pc = 2 * db + ((col & 3) >> 1);
+                        const T* const x0 = X + r0 * LD + ((pc ^ s0) << 3) + (col & 1) * 4;
+                        const T* const x1 = X + r1 * LD + ((pc ^ s1) << 3) + (col & 1) * 4;
+                        const uint2 a2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x0));
+                        const uint2 b2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)x1));
+                        o[db] = Mma<T>::run(make_uint4(a2.x, a2.y, b2.x, b2.y), p, o[db]);
+                    }
+                }
+            }
+            lds_publish_barrier();
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+                *reinterpret_cast<f32x4_t*>(parts + (wave * 16 + col) * D + 16 * db + 4 * g) = o[db];
+            lds_publish_barrier();
+#pragma unroll
+            for (int n = 0; n < kItems; ++n) {
+                const int e = tid + n * kPagedThreads, rw = e / kQuads, d = 4 * (e - rw * kQuads);
+                float mr, lr;
+                if (e >= 16 * kQuads || row0 + rw > last || !again(row0 + rw, mr, lr)) continue;
+                f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) x += *reinterpret_cast<const f32x4_t*>(parts + (w * 16 + rw) * D + d);
+                if (walk == kFinite) {
+                    sum[n] = x;
+                    continue;
+                }
+                uint32_t bits = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bits |= x[i] > 0.f ? 1u << i : 0u;
+                if (walk == kPlus) {
+                    plus[n] = bits;
+                    continue;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool up = (plus[n] >> i) & 1, down = (bits >> i) & 1;
+                    if (up || down) sum[n][i] = up && down ? __builtin_nanf("") : up ? INFINITY : -INFINITY;
+                }
+                put_four<T>(a, r, row0 + rw, d, sum[n], lr);
+            }
+            lds_publish_barrier();
+        }
+    }
+}
+
 template <typename T, int D, int NB>
 __global__ __launch_bounds__(kPagedThreads, few_waves<T>(D, NB)) void k_paged_few(PagedArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -280,6 +451,7 @@ __global__ __launch_bounds__(kPagedThreads, few_waves<T>(D, NB)) void k_paged_fe
     constexpr int kRowsOf = kFewRows * NB;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ float ml[4][kRowsOf][2];
+    __shared__ uint32_t bad[4][NB];  // rows of which a wave has a NaN among its sums
     clear_padding<T>(a);
     Share r;
     if (!find_share(a, r)) return;
@@ -471,49 +643,68 @@ __global__ __launch_bounds__(kPagedThreads, few_waves<T>(D, NB)) void k_paged_fe
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         float* const ow = parts + (wave * kRowsOf + 16 * n + col) * D;
+        float total = 0.f;
 #pragma unroll
-        for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4_t*>(ow + 16 * db + 4 * g) = o[n][db];
+        for (int db = 0; db < DB; ++db) {
+            *reinterpret_cast<f32x4_t*>(ow + 16 * db + 4 * g) = o[n][db];
+            total += (o[n][db][0] + o[n][db][1]) + (o[n][db][2] + o[n][db][3]);
+        }
         l[n] = sum_rows(l[n]);
+        unsigned long long rows = __ballot(total != total);
+        rows |= rows >> 32;
         if (g == 0) {
             ml[wave][16 * n + col][0] = m[n];
             ml[wave][16 * n + col][1] = l[n];
+            bad[wave][n] = static_cast<uint32_t>(rows | rows >> 16) & 0xffffu;
         }
     }
     lds_publish_barrier();
+    const bool any = __ballot(lane < 4 * NB && (&bad[0][0])[lane] != 0) != 0;
+    // A row's maximum and sum over the waves, each wave's weight.
+    auto joined = [&](int rw, float& mt, float& lt, float (&wt)[4]) {
+        mt = fmaxp(fmaxp(ml[0][rw][0], ml[1][rw][0]), fmaxp(ml[2][rw][0], ml[3][rw][0]));
+        const float ref = mt == -INFINITY ? 0.f : mt;
+        lt = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            wt[w] = __builtin_amdgcn_exp2f(ml[w][rw][0] - ref);
+            lt = fmaf(wt[w], ml[w][rw][1], lt);
+        }
+    };
+    // Rows to be summed again: not where the scores themselves are not finite.
+    // A row without a key (sum 0) is, to zeros.
+    auto later = [&](int rw, float mt, float lt) {
+        const int n = rw >> 4;
+        const uint32_t rows = bad[0][n] | bad[1][n] | bad[2][n] | bad[3][n];
+        return ((rows >> (rw & 15)) & 1) && (lt == 0.f || (!item_nonfinite(mt) && !item_nonfinite(lt)));
+    };
 #pragma unroll 1
     for (int e = threadIdx.x; e < r.rows * (D / 4); e += kPagedThreads) {
         const int rw = e / (D / 4), d = 4 * (e - rw * (D / 4));
-        const float mt = fmaxp(fmaxp(ml[0][rw][0], ml[1][rw][0]), fmaxp(ml[2][rw][0], ml[3][rw][0]));
-        const float ref = mt == -INFINITY ? 0.f : mt;
-        float lt = 0.f;
+        float mt, lt, wt[4];
+        joined(rw, mt, lt, wt);
         f32x4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float wt = __builtin_amdgcn_exp2f(ml[w][rw][0] - ref);
-            lt = fmaf(wt, ml[w][rw][1], lt);
-            x += wt * *reinterpret_cast<const f32x4_t*>(parts + (w * kRowsOf + rw) * D + d);
-        }
-        if (lt == 0.f) x = f32x4_t{0.f, 0.f, 0.f, 0.f};  // no key: 0 times what others see is not 0 if it is not finite
-        else if (four_nonfinite(x) && !item_nonfinite(mt) && !item_nonfinite(lt)) x = exact_four<T, D>(a, r, rw, mt, d);
-        if (r.split) {
-            const long long at = static_cast<long long>(r.index) * kRowsOf + rw;
-            *reinterpret_cast<f32x4_t*>(a.part + at * D + d) = x;
-            if (d == 0) {
+        for (int w = 0; w < 4; ++w) x += wt[w] * *reinterpret_cast<const f32x4_t*>(parts + (w * kRowsOf + rw) * D + d);
+        if (!any || !later(rw, mt, lt)) put_four<T>(a, r, rw, d, x, lt);
+        if (d == 0) {
+            if (r.split) {
+                const long long at = static_cast<long long>(r.index) * kRowsOf + rw;
                 a.ml[2 * at] = mt;
                 a.ml[2 * at + 1] = lt;
+            } else {
+                int i, hq;
+                row_token(a, r.cls, r.h, r.row0 + rw, i, hq);
+                a.lse[r.b * a.ll.b + i * a.ll.s2 + hq * a.ll.h] = row_lse(mt, lt);
             }
-            continue;
         }
-        const float inv = lt == 0.f ? 0.f : 1.f / lt;
-        int i, hq;
-        row_token(a, r.cls, r.h, r.row0 + rw, i, hq);
-        T* const out = static_cast<T*>(a.out) + r.b * a.lo.b + i * a.lo.s2 + hq * a.lo.h + d;
-        if constexpr (F32)
-            *reinterpret_cast<f32x4_t*>(out) = x * inv;
-        else
-            *reinterpret_cast<uint2*>(out) = make_uint2(Mma<T>::pack(x[0] * inv, x[1] * inv),
-                                                        Mma<T>::pack(x[2] * inv, x[3] * inv));
-        if (d == 0) a.lse[r.b * a.ll.b + i * a.ll.s2 + hq * a.ll.h] = row_lse(mt, lt);
+    }
+    if (any) {
+        redo_rows<T, D>(r, lds, [&](int rw, float& mt, float& lt) {
+            float wt[4];
+            joined(rw, mt, lt, wt);
+            return later(rw, mt, lt);
+        });
     }
 }
 
@@ -582,6 +773,8 @@ __global__ __launch_bounds__(kPagedThreads, DEPTH == 2 ? 3 : 2) void k_paged_chu
     constexpr int kTile = kChunkKeys * LD, kOffs = DEPTH + 1;
     __shared__ i64x2_t off[kOffs][kChunkKeys];  // of a key's row in the key and value pages
     __shared__ int live[kOffs][kChunkKeys];
+    __shared__ float fin[128 * QB][2];  // a row's maximum and sum, at the end
+    __shared__ uint32_t bad[4 * QB];    // rows to be summed again, 32 a word
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     T* const ks = reinterpret_cast<T*>(lds);
     T* const vs = ks + 2 * kTile;
@@ -829,50 +1022,62 @@ __global__ __launch_bounds__(kPagedThreads, DEPTH == 2 ? 3 : 2) void k_paged_chu
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
         const int rw = wrow + 32 * b + col;
-        if (rw >= r.rows) continue;
-        int qi, qh;
-        row_token(a, r.cls, r.h, r.row0 + rw, qi, qh);
         const float lt = l[b] + other_half(l[b]);
-        if (r.split) {
-            const long long at = static_cast<long long>(r.index) * a.M + rw;
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<float4*>(a.part + at * D + 8 * n + 4 * h) =
-                    make_float4(o[b][n / 4][4 * (n & 3)], o[b][n / 4][4 * (n & 3) + 1], o[b][n / 4][4 * (n & 3) + 2],
-                                o[b][n / 4][4 * (n & 3) + 3]);
-            if (h == 0) {
-                a.ml[2 * at] = m[b];
-                a.ml[2 * at + 1] = lt;
-            }
-        }
-        const float inv = lt == 0.f ? 0.f : 1.f / lt;
-        T* const out = static_cast<T*>(a.out) + r.b * a.lo.b + qi * a.lo.s2 + qh * a.lo.h;
-        if (!r.split) {
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<uint2*>(out + 8 * n + 4 * h) =
-                    make_uint2(Mma<T>::pack(o[b][n / 4][4 * (n & 3)] * inv, o[b][n / 4][4 * (n & 3) + 1] * inv),
-                               Mma<T>::pack(o[b][n / 4][4 * (n & 3) + 2] * inv, o[b][n / 4][4 * (n & 3) + 3] * inv));
-            if (h == 0) a.lse[r.b * a.ll.b + qi * a.ll.s2 + qh * a.ll.h] = row_lse(m[b], lt);
-        }
         float total = 0.f;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) total += o[b][t][i];
-        if (item_nonfinite(total) && (lt == 0.f || (!item_nonfinite(m[b]) && !item_nonfinite(lt)))) {
-            // written over, four head dims at a time; zeros where the row has no key
-#pragma unroll 1
-            for (int d = 4 * h; d < D; d += 8) {
-                f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-                if (lt != 0.f) x = exact_four<T, D>(a, r, rw, m[b], d);
-                if (r.split)
-                    *reinterpret_cast<f32x4_t*>(a.part + (static_cast<long long>(r.index) * a.M + rw) * D + d) = x;
-                else
-                    *reinterpret_cast<uint2*>(out + d) = make_uint2(Mma<T>::pack(x[0] * inv, x[1] * inv),
-                                                                    Mma<T>::pack(x[2] * inv, x[3] * inv));
+        // Rows to be summed again: not where the scores themselves are not
+        // finite.  A row without a key (sum 0) is, to zeros.
+        unsigned long long later = __ballot(total != total);
+        later |= later >> 32 | later << 32;
+        later &= __ballot(rw < r.rows && (lt == 0.f || (!item_nonfinite(m[b]) && !item_nonfinite(lt))));
+        if (h == 0) {
+            fin[rw][0] = m[b];
+            fin[rw][1] = lt;
+            bad[QB * wave + b] = static_cast<uint32_t>(later);
+        }
+        if (rw >= r.rows) continue;
+        int qi, qh;
+        row_token(a, r.cls, r.h, r.row0 + rw, qi, qh);
+        if (h == 0) {
+            if (r.split) {
+                const long long at = static_cast<long long>(r.index) * a.M + rw;
+                a.ml[2 * at] = m[b];
+                a.ml[2 * at + 1] = lt;
+            } else {
+                a.lse[r.b * a.ll.b + qi * a.ll.s2 + qh * a.ll.h] = row_lse(m[b], lt);
             }
         }
+        if ((later >> lane) & 1) continue;
+        if (r.split) {
+            float* const part = a.part + (static_cast<long long>(r.index) * a.M + rw) * D + 4 * h;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float4*>(part + 8 * n) =
+                    make_float4(o[b][n / 4][4 * (n & 3)], o[b][n / 4][4 * (n & 3) + 1], o[b][n / 4][4 * (n & 3) + 2],
+                                o[b][n / 4][4 * (n & 3) + 3]);
+            continue;
+        }
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        T* const out = static_cast<T*>(a.out) + r.b * a.lo.b + qi * a.lo.s2 + qh * a.lo.h + 4 * h;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<uint2*>(out + 8 * n) =
+                make_uint2(Mma<T>::pack(o[b][n / 4][4 * (n & 3)] * inv, o[b][n / 4][4 * (n & 3) + 1] * inv),
+                           Mma<T>::pack(o[b][n / 4][4 * (n & 3) + 2] * inv, o[b][n / 4][4 * (n & 3) + 3] * inv));
+    }
+    lds_publish_barrier();
+    uint32_t any = 0;
+#pragma unroll
+    for (int n = 0; n < 4 * QB; ++n) any |= bad[n];
+    if (__builtin_amdgcn_readfirstlane(any)) {
+        redo_rows<T, D>(r, lds, [&](int rw, float& mt, float& lt) {
+            mt = fin[rw][0];
+            lt = fin[rw][1];
+            return ((bad[rw >> 5] >> (rw & 31)) & 1) != 0;
+        });
     }
 }
 

@@ -1,10 +1,11 @@
 """Attention over a paged cache where its arithmetic has edges: values that are
-not finite beside rows that do not attend to them, and windows of any length
-beside tokens before the sequence.  Tolerances are those of
-``test_hip_paged``."""
+not finite, beside rows that do not attend to them and in long runs of keys,
+and windows of any length beside tokens before the sequence.  Tolerances are
+those of ``test_hip_paged``."""
 from __future__ import annotations
 
 import math
+import time
 
 import pytest
 import torch
@@ -102,6 +103,51 @@ def test_rows_without_a_key_beside_others(new, hq, dtype):
     got = p.run(2)
     check_rows(got, p, 0, range(new), 2)
     assert (got[1][0, :196 - first] == -math.inf).all()
+
+
+def _seconds(fn, n=3):
+    fn()
+    torch.cuda.synchronize()
+    t = time.perf_counter()
+    for _ in range(n):
+        fn()
+    torch.cuda.synchronize()
+    return (time.perf_counter() - t) / n
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new, length, kernel", [(4, 2000, None), (512, 2000, None), (512, 2000, 600)])
+def test_nonfinite_values_cost_a_few_walks(new, length, kernel, dtype):
+    """A value at an early key that is not finite, seen by all or by some
+    rows of a tile: the rows that are summed again cost a few more walks over
+    the keys, not a dot product for each head dim."""
+    p = Problem([(new, length)], 4, 2, 128, 16, dtype)
+    plain = _seconds(lambda: p.run(kernel))
+    p.vp[_at(p, 0, length - new - 100)] = math.inf
+    p.vp[_at(p, 0, length - 1)] = math.nan
+    got = p.run(kernel)
+    check_rows(got, p, 0, sorted({0, 1, new // 2, new - 1}), kernel)
+    assert _seconds(lambda: p.run(kernel), 1) <= 30 * plain + 1e-3
+
+
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+@pytest.mark.parametrize("new, length, hq, hkv, dim, kernel, dil", [
+    (6, 90, 4, 2, 64, 30, 1), (6, 90, 4, 2, 128, 30, 2), (90, 200, 4, 2, 64, 40, 1), (90, 200, 4, 2, 128, 40, 1),
+    (90, 200, 4, 2, 96, None, 1), (90, 200, 4, 2, 32, 11, 3), (40, 5000, 2, 2, 64, 3000, 1), (90, 5000, 2, 1, 64, 3000, 1),
+])
+def test_nonfinite_values_key_by_key(new, length, hq, hkv, dim, kernel, dil, dtype):
+    """Infinities of both signs and NaN at keys that some tokens attend to
+    and others do not, in dims of their own and in shared ones."""
+    p = Problem([(new, length), (3, 40)], hq, hkv, dim, 16, dtype)
+    for j, d, bad in ((length - 1, 0, math.inf), (length - new, 1, -math.inf), (length - new // 2, 2, math.nan),
+                      (length - new // 3, 3, math.inf), (length - 2, 3, -math.inf), (length - new // 2, 17, -math.inf),
+                      (length - new // 3, 17, -math.inf), (0, dim - 1, math.inf)):
+        pg, slot = _at(p, 0, j)
+        p.vp[pg, slot, 0, d] = bad
+    got = p.run(kernel, dil)
+    check_rows(got, p, 0, range(new) if length < 1000 else range(0, new, 7), kernel, dil)
+    check_rows(got, p, 1, range(3), kernel, dil)
+    assert all(torch.equal(a.nan_to_num(nan=9.0), b.nan_to_num(nan=9.0)) for a, b in zip(p.run(kernel, dil), got))
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
