@@ -173,9 +173,20 @@ __device__ __forceinline__ int piece_swz(int row) {
 
 // A row's running maximum is raised, and what was summed scaled down, only
 // where the scores pass it by this many powers of two: early keys seldom hold
-// the maximum, and exponentials up to 2^8 lose nothing (fp16 holds 2^15, a
-// sum in fp32 of 2^31 of them is far from its limit).
+// the maximum, and exponentials up to 2^8 lose nothing (a sum in fp32 of 2^31
+// of them is far from its limit).
 constexpr float kSlack = 8.f;
+
+// 16-bit probabilities are rounded once for the product with the values, the
+// matrix operands' type; sums and results stay in fp32.  A half step of the
+// type on each, against the one on the result, takes errors against 64 bits
+// to 1.2 to 1.4 times those of the 32-bit form; a second term would double
+// the products.  fp16 ones carry a factor of 2^7 (running values are relative
+// to the maximum less 7): with the slack they end at 2^15, and it is those
+// below 2^-32 of the largest that vanish, 2^-15 of the weight over 2^17 keys,
+// not those below 2^-25.  bf16 has fp32's range.
+template <typename T>
+constexpr float kCarry = std::is_same<T, f16>::value ? 7.f : 0.f;
 
 // The scale's sign goes into the queries (exact), a scale of zero makes them
 // zero, so that scores times `sc2` > 0 order as the logits do.
@@ -590,9 +601,9 @@ __global__ __launch_bounds__(kPagedThreads, few_waves<T>(D, NB)) void k_paged_fe
             else
                 top = fmaxp(fmaxp(s[n][0][0], s[n][0][1]), fmaxp(s[n][0][2], s[n][0][3]));
             top = max_rows(top) * sp.sc2;
-            const bool raise = top > m[n] + kSlack;
+            const bool raise = top > m[n] + (kSlack + kCarry<T>);
             if (__ballot(raise)) {
-                const float m2 = raise ? top : m[n];
+                const float m2 = raise ? top - kCarry<T> : m[n];
                 const float keep = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - m2);
                 m[n] = m2;
                 l[n] *= keep;
@@ -965,9 +976,9 @@ __global__ __launch_bounds__(kPagedThreads, DEPTH == 2 ? 3 : 2) void k_paged_chu
 #pragma unroll
                 for (int i = 1; i < 16; ++i) top = fmaxp(top, fmaxp(s[b][0][i], s[b][1][i]));
                 top = fmaxp(top, other_half(top)) * sp.sc2;
-                const bool raise = top > m[b] + kSlack;
+                const bool raise = top > m[b] + (kSlack + kCarry<T>);
                 if (__ballot(raise)) {
-                    const float m2 = raise ? top : m[b];
+                    const float m2 = raise ? top - kCarry<T> : m[b];
                     const float keep = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[b] - m2);
                     m[b] = m2;
                     l[b] *= keep;
