@@ -1,7 +1,8 @@
 """Attention over a paged cache where its arithmetic has edges: values that are
 not finite, beside rows that do not attend to them and in long runs of keys,
-windows of any length beside tokens before the sequence, and probabilities far
-below the largest one.  Tolerances are those of ``test_hip_paged``."""
+windows of any length beside tokens before the sequence, probabilities far
+below the largest one, and instances of the kernels that the ordinary cases do
+not reach.  Tolerances are those of ``test_hip_paged``."""
 from __future__ import annotations
 
 import math
@@ -189,3 +190,35 @@ def test_probabilities_far_below_the_largest(new, dim):
     for seq in (0, B - 1):
         check_rows(got, p, seq, sorted({0, new - 1}), slack=length * 2.0 ** -32 * p.vp.abs().max().item(),
                    lse_slack=length * 2.0 ** -24)
+
+
+# rows (new, length), heads q/kv, dim, page, kernel, dilation, dtype
+INSTANCES = {
+    "chunk_dim96": ([(129, 200), (40, 300)], 4, 2, 96, 16, None, 1, BF),
+    "chunk_dim96_window": ([(129, 200), (40, 300)], 4, 2, 96, 8, 37, 1, FP),
+    "chunk_dim96_cut": ([(40, 4500)], 2, 1, 96, 64, None, 1, FP),
+    "chunk_dim32": ([(150, 150), (97, 400)], 4, 2, 32, 16, None, 1, BF),
+    "chunk_dim32_window": ([(150, 150), (97, 400)], 4, 1, 32, 5, 50, 1, FP),
+    "chunk_dim32_cut": ([(70, 4500)], 2, 1, 32, 64, 4200, 1, BF),
+    "few_dim64_four": ([(5, 700), (4, 300)], 8, 1, 64, 64, None, 1, FP),
+    "few_dim64_four_cut": ([(5, 9000), (5, 31)], 8, 1, 64, 64, None, 1, FP),
+    "few_dim64_four_bf16": ([(60, 90), (33, 200)], 2, 2, 64, 16, 41, 1, BF),
+    "few_dim64_two": ([(5, 700), (4, 300)], 8, 2, 64, 16, None, 1, BF),
+    "few_dim96_two": ([(5, 700), (4, 300)], 8, 2, 96, 16, None, 1, BF),
+    "few_dim96_two_window": ([(30, 200), (17, 40)], 2, 2, 96, 16, 21, 1, FP),
+    "few_dim128_two": ([(5, 700), (4, 300)], 8, 2, 128, 16, None, 1, FP),
+    "few_dim128_two_cut": ([(5, 9000), (2, 5)], 8, 2, 128, 32, None, 1, BF),
+    "few_fp32_dim128_one": ([(2, 300), (1, 77)], 8, 2, 128, 16, None, 1, F32),
+    "few_fp32_dim128_one_cut": ([(2, 5000), (1, 77)], 4, 2, 128, 16, None, 1, F32),
+    "few_fp32_dim64_one": ([(1, 700), (1, 64)], 16, 2, 64, 16, 300, 1, F32),
+    "few_fp32_dim64_two": ([(5, 700), (4, 300)], 8, 2, 64, 16, None, 1, F32),
+    "few_fp32_dim96_one": ([(2, 300), (1, 77)], 8, 2, 96, 24, None, 1, F32),
+    "few_fp32_dim32_one": ([(2, 300), (1, 77)], 8, 2, 32, 16, None, 1, F32),
+}
+
+
+@pytest.mark.parametrize("name", INSTANCES)
+def test_instances_against_float64(name):
+    rows, hq, hkv, dim, page, kernel, dil, dtype = INSTANCES[name]
+    p = Problem(rows, hq, hkv, dim, page, dtype, seed=len(name))
+    check(p.run(kernel, dil), p, kernel, dil, what=name)
