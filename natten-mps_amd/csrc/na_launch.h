@@ -110,6 +110,17 @@ hipError_t paged_forward(const PagedCall& c, hipStream_t s);
 
 namespace na {
 
+// A launch has fewer than 2^32 threads along x: grids of more workgroups than
+// kGridRow (2^31 threads of 256) continue along y.  Workgroups past `blocks`
+// in the last row find nothing to do.
+constexpr int kLogGridRow = 23;
+inline dim3 wide_grid(long long blocks) {
+    constexpr long long row = 1ll << kLogGridRow;
+    return blocks <= row ? dim3(static_cast<unsigned>(blocks))
+                         : dim3(static_cast<unsigned>(row), static_cast<unsigned>((blocks + row - 1) >> kLogGridRow));
+}
+__device__ __forceinline__ int wide_block() { return static_cast<int>((blockIdx.y << kLogGridRow) + blockIdx.x); }
+
 // While a NoDeviceAlloc object lives on a thread, launches from that thread
 // allocate no device memory: the tile kernels read a geometry table only if
 // one was already built for the shape and otherwise compute the geometry

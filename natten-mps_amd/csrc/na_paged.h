@@ -131,7 +131,7 @@ __device__ __forceinline__ T lane_value(T v, int lane) {
 // no barriers, and what comes out is uniform.
 __device__ __forceinline__ bool find_share(const PagedArgs& a, Share& r) {
     const int lane = threadIdx.x & 63, target = 1 << a.log_target;
-    int want = blockIdx.x;
+    int want = wide_block();
     if (a.xcd_run) {
         // workgroups are dealt to the 8 XCDs in turn: give each XCD runs of
         // consecutive shares, whose tiles read the same keys
@@ -174,7 +174,7 @@ __device__ __forceinline__ bool find_share(const PagedArgs& a, Share& r) {
         }
         const bool cut = all < target;
         chunk = imax(static_cast<int>(__builtin_ldexpf(work, -a.log_target)) + 1, a.least);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = cut ? all : 0;
+        if (want == 0 && threadIdx.x == 0) *a.count = cut ? all : 0;
         // the sequence whose shares hold `want`.  Where keys are cut there are
         // fewer than 2^9 tiles and 2^10 shares, summed together.
         int base = 0, owner = -1, lo = 0, ns = 1;

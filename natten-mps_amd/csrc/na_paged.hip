@@ -31,7 +31,7 @@ template <typename T>
 __device__ __forceinline__ void clear_padding(const PagedArgs& a) {
     if (!a.news) return;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kPagedThreads / 64) + (threadIdx.x >> 6));
+    const int wave = __builtin_amdgcn_readfirstlane(wide_block() * (kPagedThreads / 64) + static_cast<int>(threadIdx.x >> 6));
     const int first = wave * a.per_wave, end = imin(first + a.per_wave, a.B * a.L);
     for (int t0 = first; t0 < end; t0 += 64) {
         const int t = t0 + lane;
@@ -1294,7 +1294,7 @@ constexpr size_t few_lds(int blocks) {
 
 template <typename T, int D>
 hipError_t launch_mfma(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
-    const dim3 grid(p.grid), block(kPagedThreads);
+    const dim3 grid = wide_grid(p.grid), block(kPagedThreads);
     if constexpr (!std::is_same<T, float>::value) {
         if (p.kind == kChunk) {
             constexpr int lds = 2 * 2 * kChunkKeys * row_elems<D>() * sizeof(T);
@@ -1328,9 +1328,9 @@ hipError_t launch_kind(const PagedArgs& a, const PagedPlan& p, bool vec, hipStre
     if (p.kind == kRows) {
         constexpr int kVec = 16 / sizeof(T);
         if (vec)
-            NA_LAUNCH("na_paged_rows", (k_paged_rows<T, kVec>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
+            NA_LAUNCH("na_paged_rows", (k_paged_rows<T, kVec>), wide_grid(p.grid), dim3(kPagedThreads), 0, s, a);
         else
-            NA_LAUNCH("na_paged_rows", (k_paged_rows<T, 1>), dim3(p.grid), dim3(kPagedThreads), 0, s, a);
+            NA_LAUNCH("na_paged_rows", (k_paged_rows<T, 1>), wide_grid(p.grid), dim3(kPagedThreads), 0, s, a);
         e = hipGetLastError();
     } else {
         if (a.Dqk == 32) e = launch_mfma<T, 32>(a, p, s);

@@ -176,7 +176,8 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
     __shared__ long long off[kMaxTokens][6];
     __shared__ int coord[kMaxTokens][3];  // paged: coord[.][0] is the position
     const int tid = threadIdx.x;
-    const int t0 = blockIdx.x * a.tb;
+    const int t0 = wide_block() * a.tb;
+    if (t0 >= a.tokens) return;
     const int nt = imin(a.tb, a.tokens - t0);
 
     for (int t = tid; t < nt; t += kThreads) {
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(kThreads) void k_rotary(RotaryArgs a) {
 
 template <typename T, int VEC, bool PAGED>
 hipError_t launch(const RotaryArgs& a, bool inter, bool stream, hipStream_t s) {
-    const dim3 grid((a.tokens + a.tb - 1) / a.tb), block(kThreads);
+    const dim3 grid = wide_grid((static_cast<long long>(a.tokens) + a.tb - 1) / a.tb), block(kThreads);
     const size_t shm = sizeof(float) * 2 * static_cast<size_t>(a.tb) * a.half;
     const char* const name = PAGED ? "na_paged_append" : "na_rotary";
     if constexpr (VEC > 1) {

@@ -1,8 +1,9 @@
 """Attention over a paged cache where its arithmetic has edges: values that are
 not finite, beside rows that do not attend to them and in long runs of keys,
 windows of any length beside tokens before the sequence, probabilities far
-below the largest one, and instances of the kernels that the ordinary cases do
-not reach.  Tolerances are those of ``test_hip_paged``."""
+below the largest one, instances of the kernels that the ordinary cases do not
+reach, and more tiles than a row of a grid takes.  Tolerances are those of
+``test_hip_paged``."""
 from __future__ import annotations
 
 import math
@@ -11,6 +12,7 @@ import time
 import pytest
 import torch
 
+import natten_mps_amd as na
 from test_hip_paged import BF, DEV, F32, FP, Problem, check
 
 pytestmark = pytest.mark.gpu
@@ -222,3 +224,23 @@ def test_instances_against_float64(name):
     rows, hq, hkv, dim, page, kernel, dil, dtype = INSTANCES[name]
     p = Problem(rows, hq, hkv, dim, page, dtype, seed=len(name))
     check(p.run(kernel, dil), p, kernel, dil, what=name)
+
+
+@pytest.mark.parametrize("tokens, dim, kernel, dil", [
+    (2 ** 26, 8, 1, 1),        # 2^24 tiles of four rows
+    (2 ** 24, 32, 2, 2 ** 24),  # a dilation that leaves each token alone: 2^24 tiles
+])
+def test_more_tiles_than_one_grid_row(tokens, dim, kernel, dil):
+    """A launch has fewer than 2^32 threads along x.  Each token sees itself
+    alone here: its own value comes out, and its logit as lse."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, v = (torch.randn(1, tokens, 1, dim, generator=g, device=DEV, dtype=BF) for _ in range(3))
+    pages = tokens // 64
+    table = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    lens = torch.tensor([tokens], dtype=torch.int32, device=DEV)
+    out, lse = na.na1d_paged(q, k.view(pages, 64, 1, dim), v.view(pages, 64, 1, dim), table, lens, kernel, dil,
+                             return_lse=True)
+    assert torch.equal(out, v)
+    for part in (slice(0, 4096), slice(tokens // 2 - 99, tokens // 2 + 99), slice(tokens - 4096, None)):
+        s = (q[:, part].float() * k[:, part].float()).sum(-1) * dim ** -0.5
+        assert torch.allclose(lse[:, part], s, atol=1e-5, rtol=1e-5)
