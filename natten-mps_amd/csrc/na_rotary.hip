@@ -398,7 +398,8 @@ hipError_t launch_any(RotaryArgs& a, int dtype, int vec, bool inter, int dim_v, 
     // if a store instruction writes runs of 64 bytes: 168 MB at heads of 64
     // (runs of 64) 36 -> 31 us, 205 MB interleaved 44 -> 34 us; at runs of 16
     // bytes (three axes of 16 dims) it would be 31 -> 67 us.
-    const long long bytes = elem * a.tokens * (static_cast<long long>(a.hq + a.hk) * a.dim + static_cast<long long>(a.hv) * dim_v);
+    const long long bytes = static_cast<long long>(elem) * a.tokens *
+                            (static_cast<long long>(a.hq + a.hk) * a.dim + static_cast<long long>(a.hv) * dim_v);
     const int rest = a.dim - a.turned;
     const bool stream = bytes >= (32ll << 20) && (inter || a.pairs * elem >= 64) && (!rest || rest * elem >= 64);
     if (dtype == NATTEN_F32) {
