@@ -14,12 +14,13 @@ int dtype_code(at::ScalarType t) {
 }
 
 // A plain strided device tensor with elements (no subclass, no pending
-// conjugation or negation), sizes that fit the descriptors.
+// conjugation or negation, no forward-mode tangent), sizes that fit the
+// descriptors.
 bool plain(const at::Tensor& t) {
     if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.numel() == 0) return false;
     const auto ks = t.unsafeGetTensorImpl()->key_set();
     if (ks.has(c10::DispatchKey::Python) || ks.has(c10::DispatchKey::FuncTorchBatched) ||
-        ks.has(c10::DispatchKey::FuncTorchGradWrapper) || t.is_conj() || t.is_neg())
+        ks.has(c10::DispatchKey::FuncTorchGradWrapper) || t.is_conj() || t.is_neg() || t._fw_grad(0).defined())
         return false;
     for (int64_t n : t.sizes())
         if (n > INT32_MAX) return false;

@@ -15,7 +15,8 @@ position past the table's width: tokens there are not written, and no query
 attends to them.  A page that takes new tokens must belong to one sequence;
 pages that are only read may be shared.
 
-These calls have no gradients: they refuse tensors that need them.
+These calls have no gradients: they refuse tensors that need them, or carry
+forward-mode tangents.
 """
 from __future__ import annotations
 
@@ -24,7 +25,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from natten_mps_amd._core import ops
-from natten_mps_amd.positions import RotaryPlan, check_plan
+from natten_mps_amd.positions import RotaryPlan, check_plan, has_tangent
 from natten_mps_amd.utils.params import normalize_kernel_size, normalize_tuple_param
 
 _INTS = (torch.int32, torch.int64)
@@ -47,6 +48,8 @@ def _call(name: str, x):
 def _no_grad(what: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradients: call it under torch.no_grad() or detach its tensors.")
+    if has_tangent(*tensors):
+        raise RuntimeError(f"{what} has no gradients: it takes no dual tensors (forward-mode differentiation).")
 
 
 def _check_cache(what, batch, tokens, key_pages, value_pages, block_table, seq_lens, new_lens) -> None:

@@ -5,7 +5,7 @@ A pair ``(u, v)`` of a head at coordinate ``x`` turns by the angle
 u sin t + v cos t)``.  :class:`RotaryPlan` holds the frequencies, which dims
 turn and how they pair; :func:`rotary` and :func:`rotary_qk` turn tensors in
 the package's layout ``[B, *spatial, heads, dim]``, with gradients (the map's
-transpose, the same turn backwards).
+transpose, the same turn backwards) and forward-mode tangents.
 
 On a grid each axis owns an equal share of the turned dims, and a token's
 coordinates are its indices::
@@ -24,6 +24,7 @@ import math
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from natten_mps_amd._core import ops
 
@@ -202,15 +203,18 @@ def _check_positions(positions, plan, shape) -> None:
 
 class _RotaryFunction(torch.autograd.Function):
     """Turn by the positions' angles (backwards when ``inverse``); the
-    gradient is the opposite turn, through this Function again."""
+    gradient is the opposite turn, through this Function again, a tangent
+    turns as the tensor does."""
 
     @staticmethod
     def forward(ctx, hook, plan, positions, inverse, *tensors):
         ctx.set_materialize_grads(False)
         ctx.hook, ctx.plan, ctx.inverse = hook, plan, inverse
+        ctx.like = [(t.shape, t.dtype, t.device) for t in tensors]
         ctx.explicit = positions is not None
         if ctx.explicit:
             ctx.save_for_backward(positions)
+            ctx.save_for_forward(positions)
         return tuple(hook(*tensors, *(None,) * (2 - len(tensors)), plan, positions, inverse)[:len(tensors)])
 
     @staticmethod
@@ -220,6 +224,21 @@ class _RotaryFunction(torch.autograd.Function):
         if given:
             given = list(_RotaryFunction.apply(ctx.hook, ctx.plan, positions, not ctx.inverse, *given))
         return (None, None, None, None, *(None if g is None else given.pop(0) for g in grads))
+
+    @staticmethod
+    def jvp(ctx, _hook, _plan, _positions, _inverse, *tangents):
+        positions = ctx.saved_tensors[0] if ctx.explicit else None
+        given = [t for t in tangents if t is not None]
+        given = list(_turn(ctx.hook, ctx.plan, positions, ctx.inverse, *given))
+        # autograd wants a tangent of each output
+        return tuple(torch.zeros(shape, dtype=dtype, device=device) if t is None else given.pop(0)
+                     for t, (shape, dtype, device) in zip(tangents, ctx.like))
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors (None: absent) is a dual tensor of
+    forward-mode differentiation."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _hook():
@@ -238,11 +257,10 @@ def _call(x, key, plan, positions):
     return None if fn is None else fn(x, key, plan, positions)
 
 
-def _turn(plan, positions, *tensors):
-    hook = _hook()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return _RotaryFunction.apply(hook, plan, positions, False, *tensors)
-    return hook(*tensors, *(None,) * (2 - len(tensors)), plan, positions, False)[:len(tensors)]
+def _turn(hook, plan, positions, inverse, *tensors):
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or has_tangent(*tensors):
+        return _RotaryFunction.apply(hook, plan, positions, inverse, *tensors)
+    return hook(*tensors, *(None,) * (2 - len(tensors)), plan, positions, inverse)[:len(tensors)]
 
 
 def rotary(x: torch.Tensor, plan: RotaryPlan, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -258,7 +276,7 @@ def rotary(x: torch.Tensor, plan: RotaryPlan, positions: Optional[torch.Tensor] 
     _check_tensor(x, "a tensor")
     check_plan(plan, x.shape[-1])
     _check_positions(positions, plan, x.shape)
-    return _turn(plan, positions, x)[0]
+    return _turn(_hook(), plan, positions, False, x)[0]
 
 
 def rotary_qk(query: torch.Tensor, key: torch.Tensor, plan: RotaryPlan,
@@ -274,7 +292,7 @@ def rotary_qk(query: torch.Tensor, key: torch.Tensor, plan: RotaryPlan,
         raise ValueError(f"query and key must match but for their heads: {tuple(query.shape)}, {tuple(key.shape)}.")
     check_plan(plan, query.shape[-1])
     _check_positions(positions, plan, query.shape)
-    return tuple(_turn(plan, positions, query, key))
+    return tuple(_turn(_hook(), plan, positions, False, query, key))
 
 
 __all__ = ["RotaryPlan", "rotary", "rotary_qk"]

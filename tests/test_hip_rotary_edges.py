@@ -1,9 +1,10 @@
-"""Rotary positions at the edges of their launch: more tokens than one row of
-a grid takes."""
+"""Rotary positions at their edges: more tokens than one row of a grid takes, and
+forward-mode differentiation."""
 from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import natten_mps_amd as na
 
@@ -25,3 +26,26 @@ def test_more_blocks_than_one_grid_row():
         part = slice(lo, lo + 1000)
         want = na.rotary(x[:, part], plan, torch.arange(lo, lo + 1000, device=DEV))
         assert torch.equal(out[:, part], want)
+
+
+def test_forward_mode():
+    """A dual tensor's tangent turns as the tensor does; the paged calls have
+    no gradients and refuse it."""
+    plan = na.RotaryPlan(16)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, dq, dk = (torch.randn(2, 5, h, 16, generator=g, device=DEV) for h in (4, 2, 4, 2))
+    with forward_ad.dual_level():
+        oq, ok = na.rotary_qk(forward_ad.make_dual(q, dq), k, plan)
+        value, tangent = forward_ad.unpack_dual(oq)
+        assert torch.equal(value, na.rotary(q, plan)) and torch.equal(tangent, na.rotary(dq, plan))
+        assert torch.equal(ok, na.rotary(k, plan)) and not forward_ad.unpack_dual(ok).tangent.any()
+        out = na.rotary(forward_ad.make_dual(k, dk), plan, torch.arange(5, device=DEV) + 3)
+        want = na.rotary(dk, plan, torch.arange(5, device=DEV) + 3)
+        assert torch.equal(forward_ad.unpack_dual(out).tangent, want)
+        pages = torch.zeros(4, 4, 2, 16, device=DEV)
+        table = torch.arange(4, dtype=torch.int32, device=DEV).view(2, 2)
+        lens = torch.full((2,), 5, dtype=torch.int32, device=DEV)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="dual tensors"):
+            na.na1d_paged(forward_ad.make_dual(q, dq), pages, pages, table, lens)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="dual tensors"):
+            na.na1d_paged_append(forward_ad.make_dual(k, dk), k, pages, pages.clone(), table, lens)

@@ -1,0 +1,68 @@
+"""Rotary positions and the paged cache under the program around them, without
+a GPU: forward-mode differentiation."""
+from __future__ import annotations
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import natten_mps_amd as na
+from natten_mps_amd import positions as positions_module
+from test_rotary_cpu import _cache_args
+
+
+def turn(x, plan, positions, inverse):
+    """The formula for one axis of pairs (j, j + n / 2), in torch operations."""
+    f = torch.tensor(plan.frequencies, dtype=x.dtype)
+    at = torch.arange(x.shape[1]) if positions is None else positions
+    t = (at[..., None] * f * (-1 if inverse else 1))[..., None, :]
+    u, v = x[..., :plan.dim].chunk(2, -1)
+    turned = torch.cat((u * t.cos() - v * t.sin(), u * t.sin() + v * t.cos()), -1) * plan.magnitude
+    return torch.cat((turned, x[..., plan.dim:]), -1)
+
+
+@pytest.fixture
+def formula(monkeypatch):
+    """The formula in the kernels' place: as they do, it sees no gradients."""
+    def hook(q, k, plan, positions, inverse):
+        q, k = (None if t is None else forward_ad.unpack_dual(t).primal.detach() for t in (q, k))
+        return [None if t is None else turn(t, plan, positions, inverse) for t in (q, k)]
+
+    monkeypatch.setattr(positions_module, "_hook", lambda: hook)
+
+
+@pytest.mark.parametrize("explicit", [False, True])
+def test_forward_mode_carries_the_tangent(formula, explicit):
+    plan = na.RotaryPlan(8, magnitude=1.5)
+    g = torch.Generator().manual_seed(1)
+    q, k, dq, dk = (torch.randn(2, 5, h, 10, generator=g, dtype=torch.float64) for h in (3, 2, 3, 2))
+    pos = torch.arange(5) + 7 if explicit else None
+    with forward_ad.dual_level():
+        for tangents in ((dq, dk), (dq, None), (None, dk)):
+            duals = [x if d is None else forward_ad.make_dual(x, d) for x, d in zip((q, k), tangents)]
+            out = na.rotary_qk(*duals, plan, pos)
+            for o, x, d in zip(out, (q, k), tangents):
+                value, tangent = forward_ad.unpack_dual(o)
+                assert torch.equal(value, turn(x, plan, pos, False))
+                assert torch.equal(tangent, torch.zeros_like(x) if d is None else turn(d, plan, pos, False))
+        with torch.no_grad():
+            tangent = forward_ad.unpack_dual(na.rotary(forward_ad.make_dual(q, dq), plan, pos)).tangent
+        assert torch.equal(tangent, turn(dq, plan, pos, False))
+    assert torch.autograd.gradcheck(lambda a, b: na.rotary_qk(a, b, plan, pos),
+                                    (q.requires_grad_(), k.requires_grad_()), check_forward_ad=True,
+                                    check_batched_grad=False)
+
+
+@pytest.mark.parametrize("name", ["key", "value", "key_pages", "value_pages", "query"])
+def test_paged_calls_refuse_tangents(name):
+    a = _cache_args()
+    a["query"] = torch.zeros(2, 3, 4, 8)
+    with forward_ad.dual_level():
+        a[name] = forward_ad.make_dual(a[name], torch.ones_like(a[name]))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="dual tensors"):
+            na.na1d_paged_append(**a)
+        if name in ("key", "value"):
+            return
+        del a["key"], a["value"]
+        with pytest.raises(RuntimeError, match="dual tensors"):
+            na.na1d_paged(**a)
