@@ -146,7 +146,7 @@ pybind11::object rotary(const at::Tensor& q, const std::optional<at::Tensor>& k,
                         const std::optional<at::Tensor>& positions, const at::Tensor& table, int64_t turned,
                         int64_t axes, bool interleaved, double magnitude) {
     if (!plain(q) || q.dim() < 4 || q.dim() > 6 || !operand(q, q) || dtype_code(q.scalar_type()) < 0 ||
-        q.size(-1) > 256 || turned > q.size(-1))
+        q.size(-1) > 256 || turned > q.size(-1) || !plain(table))
         return pybind11::none();
     if (k.has_value()) {
         if (!operand(*k, q) || k->dim() != q.dim() || k->size(-1) != q.size(-1)) return pybind11::none();
@@ -243,7 +243,7 @@ pybind11::object paged_append(const at::Tensor& key, const at::Tensor& value, co
     if (query.has_value() && (!operand(*query, key) || query->dim() != 4 || query->size(0) != key.size(0) ||
                               query->size(1) != key.size(1) || query->size(3) != key.size(3)))
         return pybind11::none();
-    if (turns.has_value() && (axes != 1 || turned > key.size(3))) return pybind11::none();
+    if (turns.has_value() && (axes != 1 || turned > key.size(3) || !plain(*turns))) return pybind11::none();
     if (needs_grad({&key, &value, &kp, &vp, query.has_value() ? &*query : nullptr})) return pybind11::none();
     const DeviceOf dev(key);
     const natten_paged_t p = paged_problem(key, query.has_value() ? query->size(2) : 0, kp, vp, table);

@@ -150,7 +150,8 @@ class RotaryPlan:
     def table(self, device) -> torch.Tensor:
         """The frequencies on ``device``, one int64 per pair of an axis.  Made
         on the first call there (a copy that waits for the device, so not
-        during graph capture) and kept until the process ends."""
+        during graph capture) and kept until the process ends, but for those
+        that a trace makes (fake tensors, or a compiled graph's own)."""
         device = torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
@@ -161,7 +162,10 @@ class RotaryPlan:
             if t is None:
                 if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("RotaryPlan: call plan.table(device) once before a graph is captured.")
-                t = _TABLES[key] = torch.tensor(self._turns, dtype=torch.int64).to(device)
+                t = torch.tensor(self._turns, dtype=torch.int64).to(device)
+                if type(t) is not torch.Tensor or torch.compiler.is_compiling():
+                    return t
+                _TABLES[key] = t
             self._tables[device] = t
         return t
 

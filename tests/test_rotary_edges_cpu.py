@@ -1,5 +1,5 @@
 """Rotary positions and the paged cache under the program around them, without
-a GPU: forward-mode differentiation."""
+a GPU: forward-mode differentiation and traces."""
 from __future__ import annotations
 
 import pytest
@@ -66,3 +66,27 @@ def test_paged_calls_refuse_tangents(name):
         del a["key"], a["value"]
         with pytest.raises(RuntimeError, match="dual tensors"):
             na.na1d_paged(**a)
+
+
+def test_tables_of_a_trace_are_not_kept():
+    """A table made under fake tensors, or inside a compiled function, is the
+    trace's own: real calls of this and of an equal plan get real ones."""
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+
+    def plan():
+        return na.RotaryPlan(8, base=123.0)
+
+    p = plan()
+    with FakeTensorMode():
+        assert isinstance(p.table("cpu"), FakeTensor)
+    for x in (p, plan()):
+        assert type(x.table("cpu")) is torch.Tensor
+        assert x.table("cpu").tolist() == list(p._turns)
+    p = na.RotaryPlan(8, base=124.0)
+    seen = set(positions_module._TABLES)
+    out = torch.compile(lambda x: x + p.table("cpu"), backend="eager")(torch.zeros(4, dtype=torch.int64))
+    assert out.tolist() == list(p._turns)
+    assert set(positions_module._TABLES) == seen and not p._tables
+    assert p.table("cpu").tolist() == list(p._turns)
+    with FakeTensorMode():
+        assert type(p.table("cpu")) is torch.Tensor  # one that is there serves
