@@ -11,8 +11,8 @@
 //
 // Angles.  f is a 64-bit fixed-point fraction of a turn (f * 2^64 modulo 1:
 // whole turns do nothing), so p f modulo a turn is the low 64 bits of an
-// integer product: no loss at any position, 2^-64 p at most from f's own
-// rounding.  The top 32 bits split into the nearest quarter turn and a rest
+// integer product: nothing is lost but f's own rounding, 2^-65 |p| turns with
+// f the nearest such fraction.  The top 32 bits split into the nearest quarter turn and a rest
 // within an eighth, where the Taylor sums of sine (to x^9) and cosine (to
 // x^10) leave less than 3e-9 against an fp32 half step of 3e-8.
 //

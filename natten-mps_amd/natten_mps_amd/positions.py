@@ -14,13 +14,14 @@ coordinates are its indices::
     q, k = rotary_qk(q, k, plan)              # [B, D, H, W, heads, 64]
     out = na3d(q, k, v, kernel_size=(3, 7, 7))
 
-Angles are exact at any position: a frequency is kept as a 64-bit fraction of
-a turn, and its product with an integer position drops whole turns without
-rounding.
+Angles hold at any position: a frequency is kept as the nearest 64-bit
+fraction of a turn, and its product with an integer position ``p`` drops whole
+turns without rounding, so the angle is off by ``2^-65 |p|`` turns at most.
 """
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -35,6 +36,32 @@ def _number(value, name: str) -> float:
     if isinstance(value, bool) or not isinstance(value, (int, float)) or not math.isfinite(value):
         raise ValueError(f"{name} must be a finite number, got {value!r}.")
     return float(value)
+
+
+@lru_cache(maxsize=None)
+def _pi(bits: int) -> int:
+    """pi 2^bits, to a unit or two: Machin's 16 atan(1/5) - 4 atan(1/239)."""
+    one = 1 << (bits + 16)
+
+    def atan_inverse(x):
+        total = term = one // x
+        n, sign = 3, -1
+        while term:
+            term //= x * x
+            total += sign * (term // n)
+            n, sign = n + 2, -sign
+        return total
+
+    return (16 * atan_inverse(5) - 4 * atan_inverse(239)) >> 16
+
+
+def _turn_fraction(f: float) -> int:
+    """The float f, taken as it is, in turns times 2^64, to the nearest
+    integer: f / (2 pi) in integers, with bits of pi for f's own size."""
+    n, d = f.as_integer_ratio()
+    bits = 80 + max(math.frexp(f)[1], 0)
+    num, den = n << (64 + bits), 2 * d * _pi(bits)
+    return (2 * num + den) // (2 * den)
 
 
 class RotaryPlan:
@@ -110,13 +137,9 @@ class RotaryPlan:
                 f = [x * (g + (1 - g) / s) for x, g in zip(f, keep)]
         if magnitude is None:
             magnitude = 1 + 0.1 * math.log(s) if scaling == "ramp" else 1.0
-        # turns per position modulo 1, as 64-bit fractions (two's complement
-        # where torch's signed integers hold them)
-        turns = []
-        for x in f:
-            t = x / (2 * math.pi)
-            u = min(int((t - math.floor(t)) * 2.0 ** 64), 2 ** 64 - 1)
-            turns.append(u - 2 ** 64 if u >= 2 ** 63 else u)
+        # turns per position modulo 1, as 64-bit fractions (two's complement,
+        # as torch's signed integers hold them)
+        turns = [(_turn_fraction(x) + 2 ** 63) % 2 ** 64 - 2 ** 63 for x in f]
         for name, value in (("dim", dim), ("axes", axes), ("interleaved", bool(interleaved)),
                             ("magnitude", _number(magnitude, "magnitude")), ("frequencies", tuple(f)),
                             ("_turns", tuple(turns)), ("_tables", {})):

@@ -1,6 +1,10 @@
-"""Rotary positions at their edges: more tokens than one row of a grid takes, and
-forward-mode differentiation."""
+"""Rotary positions at their edges: more tokens than one row of a grid takes,
+forward-mode differentiation, and far positions against the plan's own
+frequencies."""
 from __future__ import annotations
+
+import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -49,3 +53,21 @@ def test_forward_mode():
             na.na1d_paged(forward_ad.make_dual(q, dq), pages, pages, table, lens)
         with torch.no_grad(), pytest.raises(RuntimeError, match="dual tensors"):
             na.na1d_paged_append(forward_ad.make_dual(k, dk), k, pages, pages.clone(), table, lens)
+
+
+def test_far_positions_against_the_frequencies():
+    """The angle is p f to 2^-65 |p| turns, f the plan's frequency itself;
+    cosine and sine add two half steps of fp32 and 2e-9 of their series, and
+    half a turn's last bit of the 32 that they see."""
+    pi = Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+    plan = na.RotaryPlan(16)
+    pos = [1, 10 ** 6 + 1, 2 ** 31 - 1, 2 ** 33 + 5, -(2 ** 36) - 3, 2 ** 40 + 77]
+    x = torch.zeros(1, len(pos), 1, 16, device=DEV)
+    x[..., :8] = 1  # out = (cos, sin)
+    out = na.rotary(x, plan, torch.tensor(pos, device=DEV)).cpu().double()
+    for i, n in enumerate(pos):
+        for j, f in enumerate(plan.frequencies):
+            angle = 2 * math.pi * float(n * Fraction(f) / (2 * pi) % 1)
+            bound = 2 * 2.0 ** -24 + 2e-9 + 2 * math.pi * (2.0 ** -32 + abs(n) * 2.0 ** -65)
+            assert abs(out[0, i, 0, j] - math.cos(angle)) <= bound
+            assert abs(out[0, i, 0, 8 + j] - math.sin(angle)) <= bound

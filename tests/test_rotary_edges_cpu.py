@@ -1,6 +1,9 @@
 """Rotary positions and the paged cache under the program around them, without
-a GPU: forward-mode differentiation and traces."""
+a GPU: forward-mode differentiation, traces, and how well turns hold a frequency."""
 from __future__ import annotations
+
+import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -90,3 +93,21 @@ def test_tables_of_a_trace_are_not_kept():
     assert p.table("cpu").tolist() == list(p._turns)
     with FakeTensorMode():
         assert type(p.table("cpu")) is torch.Tensor  # one that is there serves
+
+
+# 100 digits: 2^-332
+PI = Fraction("3.1415926535897932384626433832795028841971693993751058209749445923078164062862089986280348253421170679")
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_turns_are_the_nearest_fractions(sign):
+    """Each turn is f / (2 pi) modulo 1 to half of 2^-64, f the float as it
+    is: whatever its size, as far as the digits of pi here reach."""
+    freqs = [1.0, 0.25, 7.0, 1e-9, 5e-324, 2 * math.pi, 100.0, 3.0, 1e20, 2.0 ** 100, 10000.0 ** (-2 / 64), 1 / 3, 0.0,
+             1e-300, 2.0 ** 64 / math.pi, 123456.789]
+    p = na.RotaryPlan(32, frequencies=[sign * f for f in freqs])
+    for f, t in zip(p.frequencies, p._turns):
+        assert -2 ** 63 <= t < 2 ** 63
+        gap = (Fraction(t, 2 ** 64) - Fraction(f) / (2 * PI)) % 1
+        assert min(gap, 1 - gap) <= Fraction(1, 2 ** 65) + Fraction(1, 2 ** 150), f
+    assert len(na.RotaryPlan(2, frequencies=[1.7e308])._turns) == 1
