@@ -232,19 +232,23 @@ class PagedKVCache:
         for b, (t, n) in enumerate(zip(self._tables, need)):
             if len(t) + n > self.max_pages:
                 raise RuntimeError(f"PagedKVCache: sequence {b} needs {len(t) + n} pages, at most {self.max_pages}.")
-        for t, n in zip(self._tables, need):
-            t.extend(self._free.pop() for _ in range(n))
+        changed = []
+        for b, (t, n) in enumerate(zip(self._tables, need)):
+            for _ in range(n):
+                changed.append((self._entry(b, len(t)), self._free[-1]))
+                t.append(self._free.pop())
         self._lens = [a + n for a, n in zip(self._lens, counts)]
         self._new = counts
-        self._send(any(need))
+        self._send(changed)
 
     def release(self, sequence: int) -> None:
         """Give a sequence's pages back; it starts again at length 0."""
         b = self._index(sequence)
+        changed = [(self._entry(b, i), -1) for i, p in enumerate(self._tables[b]) if p >= 0]
         self._free.extend(p for p in reversed(self._tables[b]) if p >= 0)
         self._tables[b] = []
         self._lens[b] = self._new[b] = 0
-        self._send(True)
+        self._send(changed)
 
     def trim(self, kernel_size: int, dilation: int = 1) -> None:
         """Give back the pages that lie wholly behind the windows of every
@@ -253,24 +257,28 @@ class PagedKVCache:
         step's attention: the new tokens' own windows may reach further back."""
         ks = normalize_kernel_size(kernel_size, 1)[0]
         reach = (ks - 1) * normalize_tuple_param(dilation, 1, "dilation")[0]
-        changed = False
-        for t, n in zip(self._tables, self._lens):
+        changed = []
+        for b, (t, n) in enumerate(zip(self._tables, self._lens)):
             for i in range(min(max(n - reach, 0) // self.page_size, len(t))):
                 if t[i] >= 0:
                     self._free.append(t[i])
                     t[i] = -1
-                    changed = True
+                    changed.append((self._entry(b, i), -1))
         if changed:
-            self._send(True)
+            self._send(changed)
 
-    def _send(self, tables: bool) -> None:
-        rows = self._lens + self._new
-        if tables:
-            for t in self._tables:
-                rows = rows + t + [-1] * (self.max_pages - len(t))
+    def _entry(self, sequence: int, index: int) -> int:
+        """Where in the device buffer an entry of a sequence's table lies."""
+        return self._rows + sequence * self.max_pages + index
+
+    def _send(self, changed: List[Tuple[int, int]]) -> None:
+        """Lengths, and the table's entries that changed, to the device."""
         pin = self.device.type == "cuda"
-        host = torch.tensor(rows, dtype=torch.int32, pin_memory=pin)
-        self._meta[:len(rows)].copy_(host, non_blocking=pin)
+        host = torch.tensor(self._lens + self._new, dtype=torch.int32, pin_memory=pin)
+        self._meta[:self._rows].copy_(host, non_blocking=pin)
+        if changed:
+            pairs = torch.tensor(changed, dtype=torch.int64, pin_memory=pin).to(self.device, non_blocking=pin)
+            self._meta.index_copy_(0, pairs[:, 0], pairs[:, 1].to(torch.int32))
 
 
 class PagedLayer:

@@ -1,8 +1,11 @@
 """Rotary positions and the paged cache under the program around them, without
-a GPU: forward-mode differentiation, traces, and how well turns hold a frequency."""
+a GPU: forward-mode differentiation, traces, how well turns hold a frequency,
+and the bookkeeping of many pages."""
 from __future__ import annotations
 
 import math
+import random
+import time
 from fractions import Fraction
 
 import pytest
@@ -11,7 +14,7 @@ from torch.autograd import forward_ad
 
 import natten_mps_amd as na
 from natten_mps_amd import positions as positions_module
-from test_rotary_cpu import _cache_args
+from test_rotary_cpu import _cache, _cache_args, _held
 
 
 def turn(x, plan, positions, inverse):
@@ -111,3 +114,37 @@ def test_turns_are_the_nearest_fractions(sign):
         gap = (Fraction(t, 2 ** 64) - Fraction(f) / (2 * PI)) % 1
         assert min(gap, 1 - gap) <= Fraction(1, 2 ** 65) + Fraction(1, 2 ** 150), f
     assert len(na.RotaryPlan(2, frequencies=[1.7e308])._turns) == 1
+
+
+def test_cache_follows_any_order_of_calls():
+    """The device's tables and lengths against the host's lists."""
+    rng = random.Random(3)
+    c = _cache(num_pages=40, batch=4, max_pages=12)
+    for _ in range(300):
+        op = rng.random()
+        if op < 0.6:
+            try:
+                c.reserve([rng.choice((0, 0, 1, 1, 2, 9)) for _ in range(4)])
+            except RuntimeError:
+                c.release(rng.randrange(4))
+        elif op < 0.8:
+            c.trim(rng.choice((1, 3, 8)), rng.choice((1, 2)))
+        else:
+            c.release(rng.randrange(4))
+        _held(c)
+        assert c.block_table.tolist() == [t + [-1] * (12 - len(t)) for t in c._tables]
+        assert c.seq_lens.tolist() == c.lengths and c.new_lens.tolist() == c._new
+
+
+def test_cache_of_many_pages_is_quick_to_update():
+    """What a step costs goes by the sequences and the pages that change, not
+    by the table's size."""
+    c = _cache(num_pages=1 << 16, page_size=1, batch=256, max_pages=1 << 13, head_dim=1, num_kv_heads=1)
+    c.reserve(8)
+    t = time.perf_counter()
+    for _ in range(5):
+        c.reserve(1)
+    assert (time.perf_counter() - t) / 5 < 0.1
+    t = time.perf_counter()
+    c.release(7)
+    assert time.perf_counter() - t < 0.1
