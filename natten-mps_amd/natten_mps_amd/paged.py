@@ -168,7 +168,9 @@ class PagedKVCache:
     :meth:`reserve` does its bookkeeping on the host and sends the changed
     lengths and tables to the device on the current stream without waiting;
     the device tensors (``block_table``, ``seq_lens``, ``new_lens``) keep
-    their addresses, so a captured step can be replayed after it.
+    their addresses, so a captured step can be replayed after it.  It belongs
+    between the replays: neither it nor :meth:`release` and :meth:`trim` can
+    be captured.
     """
 
     def __init__(self, num_pages: int, page_size: int, batch: int, num_kv_heads: int, head_dim: int, *,
@@ -217,11 +219,17 @@ class PagedKVCache:
             raise IndexError(f"sequence {sequence} of {self.batch}.")
         return sequence
 
+    def _host_step(self, what: str) -> None:
+        # a replay would send what the host's memory holds by then
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"PagedKVCache.{what} cannot be captured into a graph: call it between replays.")
+
     def reserve(self, new_tokens: Union[int, Sequence[int]]) -> None:
         """Make room for the next ``new_tokens`` of each sequence (one number
         for all, or one each, 0 for a sequence that waits) and count them as
         the new tokens of the calls that follow.  Raises RuntimeError, and
         changes nothing, where pages run out."""
+        self._host_step("reserve")
         counts = [new_tokens] * self.batch if isinstance(new_tokens, int) else list(new_tokens)
         if len(counts) != self.batch or any(isinstance(n, bool) or not isinstance(n, int) or n < 0 for n in counts):
             raise ValueError(f"new_tokens must be a count >= 0 for each of the {self.batch} sequences.")
@@ -243,6 +251,7 @@ class PagedKVCache:
 
     def release(self, sequence: int) -> None:
         """Give a sequence's pages back; it starts again at length 0."""
+        self._host_step("release")
         b = self._index(sequence)
         changed = [(self._entry(b, i), -1) for i, p in enumerate(self._tables[b]) if p >= 0]
         self._free.extend(p for p in reversed(self._tables[b]) if p >= 0)
@@ -255,6 +264,7 @@ class PagedKVCache:
         token to come (attention with this or a smaller ``kernel_size`` and
         ``dilation``); their table entries become -1.  Call it after the
         step's attention: the new tokens' own windows may reach further back."""
+        self._host_step("trim")
         ks = normalize_kernel_size(kernel_size, 1)[0]
         reach = (ks - 1) * normalize_tuple_param(dilation, 1, "dilation")[0]
         changed = []
