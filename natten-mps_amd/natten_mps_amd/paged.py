@@ -5,9 +5,9 @@ reference).
 Token ``j`` of sequence ``b`` lies at slot ``j % page_size`` of page
 ``block_table[b, j // page_size]``; pages are ``[pages, page_size, heads_kv,
 dim]``.  ``seq_lens[b]`` counts the tokens of the sequence with the new ones
-of this call, ``new_lens[b]`` (clamped to ``[0, L]``) the new ones: token ``i``
-of the call's padded ``[B, L, heads, dim]`` tensors is at position
-``seq_lens[b] - new_lens[b] + i``.  Lengths and tables are device tensors and are never read back, so the
+of this call, ``new_lens[b]`` the new ones: token ``i`` of the call's padded
+``[B, L, heads, dim]`` tensors is at position ``seq_lens[b] - new_lens[b] +
+i``.  Lengths and tables are device tensors and are never read back, so the
 calls can be captured into a graph and replayed as the cache grows.
 
 A table entry outside ``[0, pages)`` (like -1) names no page, nor does a
@@ -299,17 +299,13 @@ class PagedLayer:
         self.key_pages, self.value_pages = cache.key_pages[index], cache.value_pages[index]
 
     def append(self, key, value, *, query=None, plan=None):
-        """:func:`na1d_paged_append` of the reserved tokens, all of them."""
+        """:func:`na1d_paged_append` of the reserved tokens."""
         c = self.cache
-        most = max(c._new)
-        if key.ndim == 4 and key.shape[1] < most:
-            raise ValueError(f"the cache has {most} new tokens of a sequence reserved, key holds {key.shape[1]}.")
         return na1d_paged_append(key, value, self.key_pages, self.value_pages, c.block_table, c.seq_lens, c.new_lens,
                                  query=query, plan=plan)
 
     def attend(self, query, kernel_size=None, dilation=1, *, scale=None, return_lse=False):
-        """:func:`na1d_paged` of the reserved tokens (or of the last ones of
-        each sequence, where query holds fewer)."""
+        """:func:`na1d_paged` of the reserved tokens."""
         c = self.cache
         return na1d_paged(query, self.key_pages, self.value_pages, c.block_table, c.seq_lens, kernel_size, dilation,
                           new_lens=c.new_lens, scale=scale, return_lse=return_lse)
