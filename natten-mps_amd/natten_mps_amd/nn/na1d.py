@@ -25,5 +25,9 @@ class NeighborhoodAttention1D(_NeighborhoodAttentionND):
             raise ValueError("a cache needs a causal module of stride 1.")
         if self.attn_drop_p > 0.0:
             raise ValueError("a cache needs attn_drop=0.")
+        # fewer would be taken for the last ones, the slots before them left as they were
+        if q.shape[1] < cache.cache.new_tokens:
+            raise ValueError(f"the cache has {cache.cache.new_tokens} new tokens of a sequence reserved, "
+                             f"x holds {q.shape[1]}.")
         turned = cache.append(k, v, query=q if self.rotary is not None else None, plan=self.rotary)
         return cache.attend(q if turned is None else turned, self.kernel_size, self.dilation, scale=self.scale)

@@ -5,9 +5,10 @@ reference).
 Token ``j`` of sequence ``b`` lies at slot ``j % page_size`` of page
 ``block_table[b, j // page_size]``; pages are ``[pages, page_size, heads_kv,
 dim]``.  ``seq_lens[b]`` counts the tokens of the sequence with the new ones
-of this call, ``new_lens[b]`` the new ones: token ``i`` of the call's padded
-``[B, L, heads, dim]`` tensors is at position ``seq_lens[b] - new_lens[b] +
-i``.  Lengths and tables are device tensors and are never read back, so the
+of this call, ``new_lens[b]`` (clamped to ``[0, L]``) the new ones: token ``i``
+of the call's padded ``[B, L, heads, dim]`` tensors is at position
+``seq_lens[b] - new_lens[b] + i``, so a call of fewer tokens than that holds
+the last ones of the sequence.  Lengths and tables are device tensors and are never read back, so the
 calls can be captured into a graph and replayed as the cache grows.
 
 A table entry outside ``[0, pages)`` (like -1) names no page, nor does a
@@ -204,6 +205,12 @@ class PagedKVCache:
     def lengths(self) -> List[int]:
         """Tokens of each sequence, as the host counts them."""
         return list(self._lens)
+
+    @property
+    def new_tokens(self) -> int:
+        """New tokens of a sequence, at most, that the last :meth:`reserve`
+        made room for."""
+        return max(self._new)
 
     @property
     def free_pages(self) -> int:

@@ -1,6 +1,6 @@
 """Rotary positions and the paged cache under the program around them, without
 a GPU: forward-mode differentiation, traces, how well turns hold a frequency,
-and the bookkeeping of many pages."""
+the bookkeeping of many pages, and inputs that do not fit what was reserved."""
 from __future__ import annotations
 
 import math
@@ -148,3 +148,14 @@ def test_cache_of_many_pages_is_quick_to_update():
     t = time.perf_counter()
     c.release(7)
     assert time.perf_counter() - t < 0.1
+
+
+def test_module_refuses_fewer_tokens_than_reserved():
+    """They would be taken for the last ones of each sequence, and the slots
+    before them would hold what was there."""
+    c = _cache()
+    c.reserve([5, 0, 4])
+    assert c.new_tokens == 5
+    m = na.NeighborhoodAttention1D(16, 2, 3, is_causal=True)
+    with torch.no_grad(), pytest.raises(ValueError, match="5 new tokens of a sequence reserved, x holds 4"):
+        m(torch.zeros(3, 4, 16), cache=c.layer(0))
