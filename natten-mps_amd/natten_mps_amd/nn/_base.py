@@ -21,6 +21,7 @@ _SHAPES = {1: "[B, L, C]", 2: "[B, H, W, C]", 3: "[B, D, H, W, C]"}
 
 class _NeighborhoodAttentionND(torch.nn.Module):
     rank = 0
+    rotary: Optional[RotaryPlan] = None  # modules saved whole before there were plans have none
 
     def __init__(self, embed_dim: int, num_heads: int, kernel_size: Union[int, Tuple[int, ...]],
                  stride: Union[int, Tuple[int, ...]] = 1, dilation: Union[int, Tuple[int, ...]] = 1,

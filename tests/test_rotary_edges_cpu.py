@@ -1,6 +1,7 @@
 """Rotary positions and the paged cache under the program around them, without
 a GPU: forward-mode differentiation, traces, how well turns hold a frequency,
-the bookkeeping of many pages, and inputs that do not fit what was reserved."""
+the bookkeeping of many pages, inputs that do not fit what was reserved, and
+modules from before there were plans."""
 from __future__ import annotations
 
 import math
@@ -159,3 +160,15 @@ def test_module_refuses_fewer_tokens_than_reserved():
     m = na.NeighborhoodAttention1D(16, 2, 3, is_causal=True)
     with torch.no_grad(), pytest.raises(ValueError, match="5 new tokens of a sequence reserved, x holds 4"):
         m(torch.zeros(3, 4, 16), cache=c.layer(0))
+
+
+def test_module_saved_before_plans(pure_backend):
+    """A module saved whole by an earlier version has no ``rotary`` of its
+    own: it runs as it did."""
+    m = na.NeighborhoodAttention1D(16, 2, 3)
+    x = torch.randn(2, 9, 16)
+    want = m(x)
+    state = m.__getstate__() if hasattr(m, "__getstate__") else m.__dict__.copy()
+    old = na.NeighborhoodAttention1D.__new__(na.NeighborhoodAttention1D)
+    old.__setstate__({n: v for n, v in state.items() if n != "rotary"})
+    assert torch.equal(old(x), want)
