@@ -929,6 +929,13 @@ def _int32(t: Optional[torch.Tensor], device) -> Optional[torch.Tensor]:
     return t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
 
 
+def _sizes_fit(*ts: Optional[torch.Tensor]) -> None:
+    """The descriptors hold sizes in 32 bits; ctypes would cut larger ones."""
+    for t in ts:
+        if t is not None and any(n > 2 ** 31 - 1 for n in t.shape):
+            raise NotImplementedError(f"natten_mps_amd 'hip' backend: a size above 2^31 - 1 in {tuple(t.shape)}.")
+
+
 def _axis_lay(t: torch.Tensor) -> "_lib.Layout":
     return _lib.layout(t, t.ndim - 3, 1)
 
@@ -966,6 +973,7 @@ def rotary(q, k, plan, positions, inverse):
     """``(q', k')``: q and k (None: absent) turned by their positions."""
     _on_device(q, k, positions)
     _same_dtype(q, k)
+    _sizes_fit(q, k)
     outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
     if q.numel() == 0 and (k is None or k.numel() == 0):
         return outs
@@ -1020,6 +1028,7 @@ def paged_append(key, value, key_pages, value_pages, table, seq_lens, new_lens, 
     """Turned keys and values into their pages; the turned query or None."""
     _on_device(key, value, key_pages, value_pages, table, seq_lens, new_lens, query)
     _same_dtype(key, value, key_pages, value_pages, query)
+    _sizes_fit(key, value, key_pages, value_pages, table, query)
     out = None if query is None else torch.empty(query.shape, dtype=query.dtype, device=query.device)
     if key.numel() == 0:
         return out
@@ -1050,6 +1059,7 @@ def paged_forward(query, key_pages, value_pages, table, seq_lens, new_lens, kern
     """``(out, lse)`` of the new tokens' queries; lse is fp32 ``[B, L, Hq]``."""
     _on_device(query, key_pages, value_pages, table, seq_lens, new_lens)
     _same_dtype(query, key_pages, value_pages)
+    _sizes_fit(query, key_pages, value_pages, table)
     dev = query.device
     B, L, Hq, _ = query.shape
     out = torch.empty((B, L, Hq, value_pages.shape[-1]), dtype=query.dtype, device=dev)

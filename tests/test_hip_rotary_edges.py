@@ -1,6 +1,6 @@
 """Rotary positions at their edges: more tokens than one row of a grid takes,
-forward-mode differentiation, and far positions against the plan's own
-frequencies."""
+forward-mode differentiation, far positions against the plan's own frequencies,
+and sizes past 32 bits."""
 from __future__ import annotations
 
 import math
@@ -71,3 +71,20 @@ def test_far_positions_against_the_frequencies():
             bound = 2 * 2.0 ** -24 + 2e-9 + 2 * math.pi * (2.0 ** -32 + abs(n) * 2.0 ** -65)
             assert abs(out[0, i, 0, j] - math.cos(angle)) <= bound
             assert abs(out[0, i, 0, 8 + j] - math.sin(angle)) <= bound
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Views without memory of their own; nothing is launched or allocated."""
+    plan = na.RotaryPlan(2)
+    x = torch.zeros(1, 1, 1, 2, device=DEV)
+    far = x.expand(1, 2 ** 32 + 5, 1, 2)
+    with pytest.raises(NotImplementedError, match="2\\^31"):
+        na.rotary(far, plan)
+    pages = x.expand(2 ** 32 + 5, 1, 1, 2)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(NotImplementedError, match="2\\^31"):
+        na.na1d_paged(x, pages, pages, table, lens)
+    with pytest.raises(NotImplementedError, match="2\\^31"):
+        na.na1d_paged(x, x, x, table.expand(1, 2 ** 32 + 5), lens)
+    with pytest.raises(NotImplementedError, match="2\\^31"):
+        na.na1d_paged_append(far, far, x.clone(), x.clone(), table, lens)
