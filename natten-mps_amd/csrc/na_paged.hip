@@ -69,8 +69,10 @@ __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -
 // A wave per row; lanes take 64 keys for the scores, then 64 head dims for
 // the products.  `VEC` elements of a key are read at once.  Head dims and
 // alignments that the MFMA kernels do not take; a row's keys are read once a
-// query head, and address arithmetic bounds it (fp32, 257 tokens in a window
-// of 63, 4 heads of 32: 19 us where k_paged_few takes 11).
+// query head and token, and address arithmetic bounds it: one token of each of
+// 16 requests of 8192 keys, 32/8 heads of 80, 1640 us (k_paged_few at 96: 93),
+// 512 tokens over 4096 keys, 16/4 heads of 80, 3830 us (k_paged_chunk at 96:
+// 53); fp32, 257 tokens in a window of 63, 4 heads of 32, 19 (k_paged_few 11).
 template <typename T, int VEC>
 __global__ __launch_bounds__(kPagedThreads) void k_paged_rows(PagedArgs a) {
     __shared__ float qs[4][256];
@@ -257,8 +259,8 @@ __device__ __forceinline__ uint4 walk_values(uint4 x, int walk) {
 // it: the next keys' loads are issued as soon as the registers are free, and
 // page numbers one step before that.  32 requests of 1 to 16385 tokens, 32/8
 // heads of 128, one new token each: 1.08 GB in 231 to 240 us (4.6 TB/s; a
-// large copy moves 4.95), in fp32 420 us (5.1 TB/s).  One request of 131070
-// tokens and 5 new ones, 8/1 heads of 64: 34 MB in 19 us, of which 11 are
+// large copy moves 5.2 to 5.4), in fp32 440 us (4.9 TB/s).  One request of
+// 131070 tokens and 5 new ones, 8/1 heads of 64: 34 MB in 18 us, of which 11 are
 // there with 600 tokens too: latency of lengths, pages, keys and parts.
 //
 // fp32 takes v_mfma 16x16x4, 16 keys at a time: element e of the 16-byte
@@ -771,7 +773,10 @@ __device__ __forceinline__ float other_half(float v) {
 // (735 to 860 TFLOP/s; a large matrix product reaches 1257 on this card, both
 // at the clock that power leaves).  Products keep the matrix cores 39 % busy
 // and the softmax the vector ALUs 45 %; the two waves of a SIMD wait for LDS
-// reads and the barrier of a tile in the rest.  DEPTH 2 keeps two tiles'
+// reads and the barrier of a tile in the rest: the four waves read 128 KB a
+// step, about as many LDS cycles as the products take.  A step of 64 keys at
+// heads of 64 takes 1.25 us where a tile has its compute unit alone, 1.57
+// where two share it, and a tile some 8 us besides.  DEPTH 2 keeps two tiles'
 // loads in flight, for tiles of one block, whose step is shorter than a trip
 // to memory.
 constexpr int kChunkKeys = 64;

@@ -21,10 +21,11 @@
 // LDS once for all heads, then walks the tokens' vectors in memory order
 // (lanes on consecutive 16-byte vectors), its first loads out before the
 // angles.  4 x 16384 tokens of 8/2 heads of 64, bf16: 31 us (5.4 TB/s); 64 x
-// 56 x 56 of 4/4 heads of 32, interleaved fp16 views: 34 us (6.1 TB/s); three
-// axes of 16 dims, 32768 tokens of 8/8 heads of 64: 31 us (4.4 TB/s); 4096
-// tokens of 4 prompts, 32/8 heads of 128, into pages: 52 us (4.8 TB/s).  A
-// large copy moves 4.95 TB/s.
+// 56 x 56 of 4/4 heads of 32, interleaved fp16 views: 33 us (6.2 TB/s); three
+// axes of 16 dims, 32768 tokens of 8/8 heads of 64: 31 us (4.3 TB/s); 4096
+// tokens of 4 prompts, 32/8 heads of 128, into pages: 53 us (4.7 TB/s).  A
+// copy of as many bytes moves 4.9 to 5.2 TB/s over buffers that no cache
+// holds, up to 8.5 over one pair that a cache does.
 #include <type_traits>
 
 #include "na_launch.h"

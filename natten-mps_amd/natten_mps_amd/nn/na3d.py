@@ -6,7 +6,8 @@ class NeighborhoodAttention3D(_NeighborhoodAttentionND):
 
     Args: embed_dim, num_heads, kernel_size, stride, dilation, is_causal,
     num_kv_heads (GQA/MQA when smaller than num_heads), qkv_bias, qk_scale,
-    attn_drop, proj_drop.
+    attn_drop, proj_drop, rotary (a RotaryPlan of 3 axes that turns queries and
+    keys).
     """
 
     rank = 3
