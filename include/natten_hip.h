@@ -406,8 +406,9 @@ int natten_hip_rotary(const natten_rotary_t *r, const uint64_t *turns,
  * new_lens[b] (clamped to [0, tokens]; NULL: `tokens`) of them are new, token
  * i of the call at position seq_lens[b] - new_lens[b] + i.  table, seq_lens
  * and new_lens are int32 device memory and read on the stream; the call never
- * waits for the device.  batch x tokens x heads_q is at most 2^27, a table
- * covers fewer than 2^31 - 4096 positions; pools may be of any size. */
+ * waits for the device.  batch x tokens x heads_q is at most 2^27, a token's
+ * heads_q x dim_v below 2^31, a table covers fewer than 2^31 - 4096
+ * positions; pools may be of any size. */
 typedef struct {
     int32_t batch;
     int32_t tokens;        /* new tokens per sequence, padded */

@@ -949,6 +949,8 @@ int make_paged(const natten_paged_t* p, na::PagedCall& c) {
     if (p->heads_q < 1) return fail(NATTEN_ERR_INVALID, "batch, tokens and heads must be >= 1");
     if (p->heads_q % p->heads_kv != 0)
         return fail(NATTEN_ERR_INVALID, "heads_q (%d) must be divisible by heads_kv (%d)", p->heads_q, p->heads_kv);
+    if (static_cast<long long>(p->heads_q) * p->dim_v > 0x7fffffffll)  // elements of a token's row
+        return fail(NATTEN_ERR_UNSUPPORTED, "heads x dim_v above 2^31 - 1");
     if (p->kernel < 0 || p->dilation < 1) return fail(NATTEN_ERR_INVALID, "kernel and dilation must be >= 1");
     if (!p->kernel && p->dilation != 1) return fail(NATTEN_ERR_INVALID, "a dilation needs a kernel");
     c.batch = p->batch;

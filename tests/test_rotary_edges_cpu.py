@@ -1,9 +1,10 @@
 """Rotary positions and the paged cache under the program around them, without
 a GPU: forward-mode differentiation, traces, how well turns hold a frequency,
-the bookkeeping of many pages, inputs that do not fit what was reserved, and
-modules from before there were plans."""
+the bookkeeping of many pages, inputs that do not fit what was reserved,
+modules from before there were plans, and limits."""
 from __future__ import annotations
 
+import ctypes
 import math
 import random
 import time
@@ -15,7 +16,8 @@ from torch.autograd import forward_ad
 
 import natten_mps_amd as na
 from natten_mps_amd import positions as positions_module
-from test_rotary_cpu import _cache, _cache_args, _held
+from natten_mps_amd._core import _lib
+from test_rotary_cpu import _cache, _cache_args, _held, _paged
 
 
 def turn(x, plan, positions, inverse):
@@ -172,3 +174,13 @@ def test_module_saved_before_plans(pure_backend):
     old = na.NeighborhoodAttention1D.__new__(na.NeighborhoodAttention1D)
     old.__setstate__({n: v for n, v in state.items() if n != "rotary"})
     assert torch.equal(old(x), want)
+
+
+def test_rows_past_31_bits_are_refused():
+    """The elements of a token's row are counted in 32 bits."""
+    lib, lay, d = _lib.load(), ctypes.byref(_lib.Layout()), ctypes.c_void_p(16)
+    p = _paged(batch=1, tokens=1, heads_q=2 ** 24, dim_v=128)
+    rc = lib.natten_hip_paged_forward(ctypes.byref(p), d, d, None, d, lay, d, d, d, lay, d, lay, None, 0, None)
+    assert rc == 2 and "heads x dim_v" in lib.natten_hip_last_error().decode()
+    assert lib.natten_hip_paged_workspace(ctypes.byref(p)) == -1
+    assert lib.natten_hip_paged_workspace(ctypes.byref(_paged(batch=1, tokens=1, heads_q=2 ** 23, dim_v=128))) >= 0
